@@ -375,15 +375,20 @@ def _attend(q, k, v, t0, first, window, softcap):
 # --------------------------------------------------------- in 64 bits
 
 
+def _pow2(e):
+    """2^e in f64, by its exponent field (torch's ldexp takes a power, which is not exact)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _stored64(x):
     """The values that the cache holds for head vectors x, from the format's definition."""
     x = x.double()
     mant, e = torch.frexp(x.abs().amax(-1, keepdim=True) / 448.0)
     e = torch.where(mant == 0.5, e - 1, e).clamp(min=-126)
-    t = torch.ldexp(x, -e)
+    t = x * _pow2(-e)
     _, te = torch.frexp(t)
-    quantum = torch.ldexp(torch.ones_like(t), (te - 1).clamp(min=-6) - 3)
-    return torch.ldexp(torch.round(t / quantum) * quantum, e)
+    quantum = _pow2((te - 1).clamp(min=-6) - 3)
+    return torch.round(t / quantum) * quantum * _pow2(e)
 
 
 def exact(case, seed):
