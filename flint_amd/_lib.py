@@ -21,7 +21,7 @@ THB_ERR_GPU = -3
 THB_ERR_INVALID = -4
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
-KV_BF16_TRUNC, KV_F16_RNE = 0, 1
+KV_BF16_TRUNC, KV_F16_RNE, KV_E4M3 = 0, 1, 2
 NO_PAGE = 0xFFFFFFFF
 SEQ_PER_ROW = 0xFFFFFFFF
 
@@ -159,6 +159,7 @@ SIGNATURES = [
     ("thb_rows_write", _int, [_vp, _pu32, _pu32, _u32, _vp]),
     ("thb_rows_device", _vp, [_vp]),
     ("thb_kv_store", _int, [_vp, _u32, _vp, _vp, _u32, _vp, _u32, _u32, _vp]),
+    ("thb_kv_load", _int, [_vp, _u32, _vp, _vp, _u32, _vp, _u32, _u32, _vp]),
     ("thb_attn", _int, [_vp, _u32, _vp, _vp, ctypes.POINTER(AttnSpecC), _vp, _vp]),
     ("thb_attn_append", _int, [_vp, _u32, _vp, _vp, _u32, _vp, _vp, ctypes.POINTER(AttnSpecC), _vp, _vp]),
     ("thb_rope_rows", _int, [_vp, _u32, _u32, _u32, _u32, _vp, ctypes.POINTER(RopeC), _vp, _u32, _vp]),

@@ -1900,7 +1900,7 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
     const uint32_t PL = pool->part_len;
     const uint32_t hd_t = template_hd(hd);
     const bool wide = prefill_wide(hd_t);
-    const uint32_t WB = block_groups(wide, hd_t);  // query groups per prefill block
+    const uint32_t WB = is_q8(pool) ? 0u : block_groups(wide, hd_t);  // query groups per prefill block
     QueryPlan qp = plan_groups(rp, G, PL, std::max<uint32_t>(pool->page_len, 16), WB);
     auto& groups = qp.groups;
     auto& blocks = qp.blocks;
@@ -2164,7 +2164,7 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
         longest = std::max<uint64_t>(longest, work(gr, 5, 6, 8, 9));
         cols = std::max(cols, gr[1] * gr[3]);
     }
-    plan.spread = n_items > 0 && n_bitems == 0 && spread_head_dim(hd, pool->page_len) &&
+    plan.spread = !is_q8(pool) && n_items > 0 && n_bitems == 0 && spread_head_dim(hd, pool->page_len) &&
                   spread_rule(hd, cols, n_items, pool->kv_heads, longest, max_parts);
     plan.merge_off = static_cast<uint32_t>(merge_off);
     plan.hd_t = hd_t;
@@ -2204,7 +2204,7 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
         std::sort(seen.begin(), seen.end());
         fuse = std::adjacent_find(seen.begin(), seen.end()) == seen.end();
     }
-    plan.fusable = fuse;
+    plan.fusable = fuse && !is_q8(pool);
     return THB_OK;
 }
 
@@ -2304,6 +2304,7 @@ void fill_args(thb_pool* pool, uint32_t layer, const thb_attn_io& io, const thb_
     a.table = pool->table_dev;
     a.k = reinterpret_cast<uint16_t*>(pool->mem + g.k_off);
     a.v = reinterpret_cast<uint16_t*>(pool->mem + g.v_off);
+    a.scales = pool->mem + g.s_off;
     a.plane = static_cast<uint64_t>(pool->arena.a.pages()) * pool->page_len * hd;
     a.max_pages = pool->arena.a.max_pages();
     a.pages = pool->arena.a.pages();
@@ -2376,7 +2377,10 @@ void launch_plan(thb_pool* pool, uint32_t layer, const thb_attn_io& io, const th
     // interleaved launch; otherwise the decode items, then the prefill
     // blocks, on the caller's stream.  (Running the prefill kernel on a
     // second stream measured slower: 262 vs 248 us per C3 layer.)
-    if (plan.mixed) {
+    if (is_q8(pool)) {
+        if (n_wg) launch_q8_decode(hd_t, dim3(static_cast<uint32_t>(n_wg)), a, s);
+        THB_HIP(hipGetLastError());
+    } else if (plan.mixed) {
         launch_mixed(hd_t, f16, plan.narrow, dim3(static_cast<uint32_t>(n_wg + n_pwg)), a, s);
         THB_HIP(hipGetLastError());
     } else if (spread) {
@@ -2386,7 +2390,7 @@ void launch_plan(thb_pool* pool, uint32_t layer, const thb_attn_io& io, const th
         launch(hd_t, f16, dim3(static_cast<uint32_t>(n_wg)), a, s);
         THB_HIP(hipGetLastError());
     }
-    if (n_pwg && !plan.mixed) {
+    if (n_pwg && !plan.mixed && !is_q8(pool)) {
         launch_prefill(hd_t, f16, plan.narrow, dim3(static_cast<uint32_t>(n_pwg)), a, s);
         THB_HIP(hipGetLastError());
     }
@@ -2651,7 +2655,7 @@ void dplan_layout(thb_dplan* p) {
     DPlanTables& t = p->tab;
     // Only a plan whose largest call could be spread holds waves: others would
     // pay for attn_pick's registers and LDS.
-    const bool small = p->gmax * pool->kv_heads <= kSpreadMax;
+    const bool small = !is_q8(pool) && p->gmax * pool->kv_heads <= kSpreadMax;
     bool other = false;
     for (const auto& g : pool->geom) {
         if (!small || !spread_head_dim(g.head_dim, pool->page_len))
@@ -2764,7 +2768,9 @@ void dplan_launch_grid(thb_pool* pool, uint32_t layer, const thb_attn_io& io, co
     const uint64_t n_wg =
         static_cast<uint64_t>(t.hd[ti] ? t.slots : plan->gmax * plan->pmax) * pool->kv_heads;
     if (n_wg > 0x7FFFFFFFull) throw HipError{hipErrorInvalidConfiguration, "attention grid too large"};
-    if (t.hd[ti])
+    if (is_q8(pool))
+        launch_q8_decode(template_hd(hd), dim3(static_cast<uint32_t>(n_wg)), a, s);
+    else if (t.hd[ti])
         launch_pick(hd, f16, dim3(static_cast<uint32_t>(n_wg)), a, s);
     else
         launch(template_hd(hd), f16, dim3(static_cast<uint32_t>(n_wg)), a, s);
@@ -2787,6 +2793,9 @@ int thb_dplan_create_ex(thb_pool* pool, uint32_t max_m, uint32_t q_heads, uint32
     const bool list = (flags & THB_DPLAN_PREFILL) != 0;
     if (list && (flags & THB_DPLAN_APPEND))
         return fail(THB_ERR_INVALID, "THB_DPLAN_APPEND takes the fixed-grid plan (without THB_DPLAN_PREFILL)");
+    if (is_q8(pool) && flags)
+        return fail(THB_ERR_CONFIG, "device plans of an 8-bit pool take no flags (fixed grid; capture thb_kv_store "
+                                    "for the append)");
     const uint32_t max_rows = list ? kDPlanListMaxRows : kDPlanMaxRows;
     if (max_m == 0 || max_m > max_rows)
         return fail(THB_ERR_INVALID, "device-planned calls take 1 to " + std::to_string(max_rows) + " rows, not " +

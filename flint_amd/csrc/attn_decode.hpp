@@ -126,12 +126,17 @@ struct AttnArgs {
     uint32_t rope_on;
     const uint32_t* meta;  // row meta of the call's rows (positions)
     RopeDev qrope, krope;
+    uint8_t* scales;  // an 8-bit pool's scales (q8.hpp); k and v then address its codes
 };
 
 // Decode items one wave per workgroup (attn_spread.hip; head_dim 64, 128 or
 // 256 exactly, pages of at least 16 tokens).
 void launch_spread(uint32_t hd, bool f16, dim3 grid, const AttnArgs& a, hipStream_t s);
 void launch_pick(uint32_t hd, bool f16, dim3 grid, const AttnArgs& a, hipStream_t s);
+
+// Decode items over an 8-bit pool (attn_q8.hip), one per workgroup; hd is the
+// head_dim template (64, 128, 256 or 512).
+void launch_q8_decode(uint32_t hd, dim3 grid, const AttnArgs& a, hipStream_t s);
 
 namespace {
 
@@ -388,36 +393,21 @@ __device__ inline void store_y(const AttnArgs& a, uint32_t row, uint32_t head, u
     }
 }
 
-// Q^T operand of a lane: column (row, head), dims 32j + 8 a4 .. + 8 of k-step
-// j, split into high and low halves.  The raw query is split (the prefill
-// kernel passes pre = the sign of the score scale, an exact multiply) and the
-// f32 scores are scaled afterwards, so the low half stays out of the f16
-// subnormal range.  In the FULL kernels: query heads q_stride apart and,
+// The query elements of a lane: column (row, head), dims 32j + 8 a4 .. + 8 of
+// k-step j, as f32.  In the FULL kernels: query heads q_stride apart and,
 // with rope on, the query head is first normalised (q_norm; the four lanes
 // of the column add their sums of squares) and rotated at the row's
 // position.  Every lane must call it (column sums).
-template <int KS, class O, bool FULL>
-__device__ inline void load_q(const AttnArgs& a, bool con, uint32_t row, uint32_t head, uint32_t a4,
-                              typename O::in8 (&qh)[KS], typename O::in8 (&ql)[KS], float pre = 1.0f) {
+template <int KS, bool FULL>
+__device__ __forceinline__ void load_q_f32(const AttnArgs& a, bool con, uint32_t row, uint32_t head, uint32_t a4,
+                                           float (&x)[KS][8]) {
     const uint32_t hd = a.head_dim;
     const uint64_t qbase = (static_cast<uint64_t>(row) * a.q_heads + head) * (FULL ? a.q_stride : hd);
-    const bool rope = FULL && a.rope_on;
-    if (!rope) {
-        float x[KS][8];
-        load_q_all<KS, FULL>(a, con, qbase, a4, x);
-#pragma unroll
-        for (int j = 0; j < KS; j++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[j][e] *= pre;
-            O::split8(x[j], qh[j], ql[j]);
-        }
-        return;
-    }
+    load_q_all<KS, FULL>(a, con, qbase, a4, x);
+    if (!FULL || !a.rope_on) return;
     // Rotary path: the lane's chunks in registers, normalised in place.
     const RopeDev& r = a.qrope;
     const uint32_t pos = con ? a.meta[8 * row] : 0u;
-    float x[KS][8];
-    load_q_all<KS, FULL>(a, con, qbase, a4, x);
     float inv = 1.0f;
     if (r.w) {
         float ss = 0.0f;
@@ -459,6 +449,17 @@ __device__ inline void load_q(const AttnArgs& a, bool con, uint32_t row, uint32_
             }
         }
     }
+}
+
+// Q^T operand of a lane (load_q_f32's elements), split into high and low
+// halves.  The raw query is split (the prefill kernel passes pre = the sign of
+// the score scale, an exact multiply) and the f32 scores are scaled afterwards,
+// so the low half stays out of the f16 subnormal range.
+template <int KS, class O, bool FULL>
+__device__ inline void load_q(const AttnArgs& a, bool con, uint32_t row, uint32_t head, uint32_t a4,
+                              typename O::in8 (&qh)[KS], typename O::in8 (&ql)[KS], float pre = 1.0f) {
+    float x[KS][8];
+    load_q_f32<KS, FULL>(a, con, row, head, a4, x);
 #pragma unroll
     for (int j = 0; j < KS; j++) {
 #pragma unroll

@@ -12,6 +12,7 @@
 #include "codec.hpp"
 #include "layout.hpp"
 #include "pool.hpp"
+#include "q8.hpp"
 #include "rope.hpp"
 
 namespace thb {
@@ -658,25 +659,62 @@ __device__ void copy_page_plane(const CopyArgs& a, const DevLayer& L, uint32_t w
     }
 }
 
+// copy_page_plane of an 8-bit pool: slots [0, ntok) of a page's codes of K or
+// V, in 16-byte units (of one slot in K, of 4 slots in V), and their scales (by
+// the workgroup of each operand).
+__device__ void copy_page_plane_q8(const CopyArgs& a, const DevLayer& L, uint32_t which, uint32_t h, uint32_t src,
+                                   uint32_t dst, uint32_t ntok) {
+    const uint32_t shift = a.page_shift, width = q8_width(L.head_dim);
+    const uint64_t head = (static_cast<uint64_t>(h) * a.pool_len) >> shift;  // the head's first page
+    uint8_t* codes = a.mem + (which ? L.v_off : L.k_off);
+    const uint8_t* sp = codes + ((head + src) << shift) * width;
+    uint8_t* dp = codes + ((head + dst) << shift) * width;
+    const uint8_t* ss = a.mem + L.s_off + ((head + src) << shift) * 2u;
+    uint8_t* ds = a.mem + L.s_off + ((head + dst) << shift) * 2u;
+    for (uint32_t t = threadIdx.x; t < ntok; t += 256) ds[q8_s_off(t, which)] = ss[q8_s_off(t, which)];
+    const uint32_t units = (width << shift) >> 4;
+    for (uint32_t u = threadIdx.x; u < units; u += 256) {
+        // unit u: tile u / width, block (u % width) / 64, lane (a, c) of it
+        const uint32_t lane = (u % width) & 63u;
+        const uint32_t slot = 16u * (u / width) + (which ? 4u * (lane >> 4) : lane & 15u);
+        if (slot >= ntok) continue;
+        const uint4 n = ld_stream16(sp + 16u * u);
+        if (!which || slot + 4u <= ntok) {
+            *reinterpret_cast<uint4*>(dp + 16u * u) = n;
+            continue;
+        }
+        const uint32_t mask = (1u << (8u * (ntok - slot))) - 1u;  // the slots below ntok, of each dim
+        uint4 o = *reinterpret_cast<const uint4*>(dp + 16u * u);
+        o.x = (o.x & ~mask) | (n.x & mask);
+        o.y = (o.y & ~mask) | (n.y & mask);
+        o.z = (o.z & ~mask) | (n.z & mask);
+        o.w = (o.w & ~mask) | (n.w & mask);
+        *reinterpret_cast<uint4*>(dp + 16u * u) = o;
+    }
+}
+
 // Grid: (x, layers * 2 * kv_heads), plane fastest.  Without a count,
 // workgroup x copies triple x; with one, the x workgroups of a plane walk
 // the *count triples of the device list (a launch sized without the host).
+template <bool Q8>
 __global__ __launch_bounds__(256) void block_copy_kernel(CopyArgs a) {
     const uint32_t planes = 2 * a.kv_heads;
     const uint32_t layer = blockIdx.y / planes, plane = blockIdx.y - layer * planes;
     const uint32_t which = plane >= a.kv_heads, h = plane - which * a.kv_heads;
     const DevLayer L = a.layers[layer];
+    auto copy = [&](const uint32_t* t) {
+        if constexpr (Q8)
+            copy_page_plane_q8(a, L, which, h, t[0], t[1], t[2]);
+        else
+            copy_page_plane(a, L, which, h, t[0], t[1], t[2]);
+    };
     if (a.count) {
         const uint32_t n = *a.count;
         for (uint32_t t = blockIdx.x; t < n; t += gridDim.x)
-            copy_page_plane(a, L, which, h, a.triples[3 * t], a.triples[3 * t + 1], a.triples[3 * t + 2]);
+            copy(a.triples + 3 * t);
         return;
     }
-    if (a.triples)
-        copy_page_plane(a, L, which, h, a.triples[3 * blockIdx.x], a.triples[3 * blockIdx.x + 1],
-                        a.triples[3 * blockIdx.x + 2]);
-    else
-        copy_page_plane(a, L, which, h, a.inl[3 * blockIdx.x], a.inl[3 * blockIdx.x + 1], a.inl[3 * blockIdx.x + 2]);
+    copy((a.triples ? a.triples : a.inl) + 3 * blockIdx.x);
 }
 
 template <uint32_t SRC>
@@ -820,6 +858,33 @@ int check_rope(const thb_rope* r, uint32_t head_dim, const thb_rows* rows, uint3
     return THB_OK;
 }
 
+int check_rows_distinct(thb_pool* p, const thb_rows* rows, uint32_t row_off, uint32_t m) {
+    if (p->distinct_rows == rows && p->distinct_version == rows->version && p->distinct_off == row_off &&
+        p->distinct_m == m)
+        return THB_OK;
+    return guarded([&]() -> int {
+        std::vector<uint64_t> at(m);
+        bool rising = true;  // the usual order: nothing to sort
+        for (uint32_t i = 0; i < m; i++) {
+            const uint32_t* r = rows->host.data() + 8 * (static_cast<size_t>(row_off) + i);
+            at[i] = (static_cast<uint64_t>(r[1]) << 32) | r[0];
+            rising = rising && (i == 0 || at[i] > at[i - 1]);
+        }
+        if (!rising) {
+            std::sort(at.begin(), at.end());
+            const auto d = std::adjacent_find(at.begin(), at.end());
+            if (d != at.end())
+                return fail(THB_ERR_INVALID, "two rows append position " + std::to_string(static_cast<uint32_t>(*d)) +
+                                                 " of sequence " + std::to_string(*d >> 32));
+        }
+        p->distinct_rows = rows;
+        p->distinct_version = rows->version;
+        p->distinct_off = row_off;
+        p->distinct_m = m;
+        return THB_OK;
+    });
+}
+
 namespace {
 // Copy arguments of pool p; the triples are set by the caller.
 CopyArgs copy_args(const thb_pool* p) {
@@ -834,15 +899,18 @@ CopyArgs copy_args(const thb_pool* p) {
 
 // Launches block_copy_kernel over n triples (a.triples on the device, or
 // a.inl), one workgroup per (triple, plane).
-void launch_copy_grid(const CopyArgs& a, uint32_t n, uint32_t layers, hipStream_t stream) {
+void launch_copy_grid(const CopyArgs& a, bool q8, uint32_t n, uint32_t layers, hipStream_t stream) {
     const uint64_t planes = static_cast<uint64_t>(layers) * 2 * a.kv_heads;
     if (planes > kMaxGridY) throw HipError{hipErrorInvalidConfiguration, "block copy: layers*2*kv_heads > 65535"};
     constexpr uint32_t kMaxGridX = 1u << 30;
     for (uint32_t i0 = 0; i0 < n; i0 += kMaxGridX) {
         CopyArgs b = a;
         if (a.triples) b.triples = a.triples + 3 * static_cast<size_t>(i0);
-        hipLaunchKernelGGL(block_copy_kernel, dim3(std::min(kMaxGridX, n - i0), static_cast<uint32_t>(planes)),
-                           dim3(256), 0, stream, b);
+        const dim3 grid(std::min(kMaxGridX, n - i0), static_cast<uint32_t>(planes));
+        if (q8)
+            hipLaunchKernelGGL(block_copy_kernel<true>, grid, dim3(256), 0, stream, b);
+        else
+            hipLaunchKernelGGL(block_copy_kernel<false>, grid, dim3(256), 0, stream, b);
         THB_HIP(hipGetLastError());
     }
 }
@@ -859,7 +927,7 @@ void launch_block_copy(thb_pool* p, const uint32_t* triples, uint32_t n, uint32_
         p->stager.upload(dev, triples, static_cast<size_t>(n) * 12, stream);
         a.triples = static_cast<const uint32_t*>(dev);
     }
-    launch_copy_grid(a, n, p->layers, stream);
+    launch_copy_grid(a, is_q8(p), n, p->layers, stream);
 }
 
 void launch_block_copy_dev(thb_pool* p, const uint32_t* triples_dev, uint32_t n, uint32_t max_tokens,
@@ -867,7 +935,7 @@ void launch_block_copy_dev(thb_pool* p, const uint32_t* triples_dev, uint32_t n,
     if (n == 0 || max_tokens == 0) return;
     CopyArgs a = copy_args(p);
     a.triples = triples_dev;
-    launch_copy_grid(a, n, p->layers, stream);
+    launch_copy_grid(a, is_q8(p), n, p->layers, stream);
 }
 
 void launch_block_copy_counted(thb_pool* p, const uint32_t* triples_dev, const uint32_t* count_dev, uint32_t grid_x,
@@ -875,7 +943,7 @@ void launch_block_copy_counted(thb_pool* p, const uint32_t* triples_dev, const u
     CopyArgs a = copy_args(p);
     a.triples = triples_dev;
     a.count = count_dev;
-    launch_copy_grid(a, std::max<uint32_t>(grid_x, 1), p->layers, stream);
+    launch_copy_grid(a, is_q8(p), std::max<uint32_t>(grid_x, 1), p->layers, stream);
 }
 
 }  // namespace thb
@@ -907,6 +975,15 @@ int thb_kv_store(thb_pool* pool, uint32_t layer, const void* k_src, const void* 
             uint32_t pos = rows->host[8 * r], seq = rows->host[8 * r + 1];
             if (int rc = check_cover(pool, seq, static_cast<uint64_t>(pos) + 1)) return rc;
         }
+    }
+    if (is_q8(pool)) {
+        if (!follow)
+            if (int rc = check_rows_distinct(pool, rows, row_off, m)) return rc;
+        return guarded([&]() -> int {
+            pool_flush(pool, as_stream(stream));
+            launch_q8_store(pool, layer, k_src, v_src, src_dtype, nullptr, rows, row_off, m, as_stream(stream));
+            return THB_OK;
+        });
     }
     return guarded([&]() -> int {
         hipStream_t s = as_stream(stream);
@@ -976,6 +1053,36 @@ int thb_kv_store(thb_pool* pool, uint32_t layer, const void* k_src, const void* 
     });
 }
 
+int thb_kv_load(thb_pool* pool, uint32_t layer, void* k_dst, void* v_dst, uint32_t dst_dtype, const thb_rows* rows,
+                uint32_t row_off, uint32_t m, void* stream) {
+    if (!pool || !rows) return fail(THB_ERR_INVALID, "null pool or rows");
+    if (!is_q8(pool))
+        return fail(THB_ERR_CONFIG, "thb_kv_load reads 8-bit pools; thb_kv_gather reads this one");
+    if (int rc = check_layer(pool, layer)) return rc;
+    if (m == 0) return THB_OK;
+    if (!k_dst || !v_dst) return fail(THB_ERR_INVALID, "null destination buffer");
+    if (dst_dtype > THB_DT_BF16) return fail(THB_ERR_INVALID, "unknown dst_dtype " + std::to_string(dst_dtype));
+    if (!aligned16(k_dst) || !aligned16(v_dst))
+        return fail(THB_ERR_INVALID, "destination buffers must be 16-byte aligned");
+    // Under capture in graph mode the call follows each replay's row meta, as thb_kv_store does.
+    const bool cap = capturing(as_stream(stream));
+    const bool follow = cap && pool->graph_mode;
+    if (static_cast<uint64_t>(row_off) + m > (follow ? rows->max_m : rows->m))
+        return fail(THB_ERR_INVALID, "row meta holds " + std::to_string(follow ? rows->max_m : rows->m) +
+                                         " rows, call needs " + std::to_string(static_cast<uint64_t>(row_off) + m));
+    if (!follow) {
+        if (!cap)
+            if (int rc = sync_mirror(pool, as_stream(stream))) return rc;
+        for (uint32_t r = row_off; r < row_off + m; r++)
+            if (int rc = check_cover(pool, rows->host[8 * r + 1], static_cast<uint64_t>(rows->host[8 * r]) + 1)) return rc;
+    }
+    return guarded([&]() -> int {
+        pool_flush(pool, as_stream(stream));
+        launch_q8_load(pool, layer, k_dst, v_dst, dst_dtype, rows, row_off, m, as_stream(stream));
+        return THB_OK;
+    });
+}
+
 // A scatter writes in place: a page another sequence also holds (a fork's
 // shared prefix) would change under it.
 static int check_unshared(const thb_pool* pool, uint32_t seq, uint32_t t0, uint32_t n) {
@@ -1014,6 +1121,9 @@ static void gather_shape(const thb_pool* pool, uint32_t hd, GatherArgs& a, size_
 static int gather_common(thb_pool* pool, uint32_t layer, uint32_t seq, uint32_t t0, uint32_t n, void* k, void* v,
                          void* stream, bool to_flat) {
     if (!pool) return fail(THB_ERR_INVALID, "pool is null");
+    if (is_q8(pool))
+        return fail(THB_ERR_CONFIG, "gather and scatter move 16-bit words; an 8-bit pool is read with thb_kv_load and "
+                                    "written with thb_kv_store");
     if (int rc = check_layer(pool, layer)) return rc;
     if (n == 0) return THB_OK;
     if (!k || !v) return fail(THB_ERR_INVALID, "null buffer");
@@ -1057,6 +1167,9 @@ static int gather_common(thb_pool* pool, uint32_t layer, uint32_t seq, uint32_t 
 static int gather_batch(thb_pool* pool, const thb_kv_range* ranges, uint32_t count, void* k, void* v, void* stream,
                         bool to_flat) {
     if (!pool) return fail(THB_ERR_INVALID, "pool is null");
+    if (is_q8(pool))
+        return fail(THB_ERR_CONFIG, "gather and scatter move 16-bit words; an 8-bit pool is read with thb_kv_load and "
+                                    "written with thb_kv_store");
     if (count == 0) return THB_OK;
     if (!ranges) return fail(THB_ERR_INVALID, "ranges is null");
     if (!k || !v) return fail(THB_ERR_INVALID, "null buffer");
@@ -1270,6 +1383,14 @@ int thb_kv_store_rope(thb_pool* pool, uint32_t layer, const void* k_src, const v
     }
     const uint64_t waves = static_cast<uint64_t>(m) * pool->kv_heads;
     if (waves > 0x7FFFFFFFull) return fail(THB_ERR_INVALID, "rotary append: m * kv_heads too large");
+    if (is_q8(pool)) {
+        if (int rc = check_rows_distinct(pool, rows, row_off, m)) return rc;
+        return guarded([&]() -> int {
+            pool_flush(pool, as_stream(stream));
+            launch_q8_store(pool, layer, k_src, v_src, src_dtype, rope, rows, row_off, m, as_stream(stream));
+            return THB_OK;
+        });
+    }
     return guarded([&]() -> int {
         hipStream_t s = as_stream(stream);
         pool_flush(pool, s);

@@ -7,6 +7,8 @@
 // (layout.hpp): K in 32-dimension groups, [head_dim / 32][page_len][32]; V
 // in 4-slot groups, [page_len / 4][head_dim][4].  Every plane is aligned to
 // 256 bytes.
+// An 8-bit pool holds per layer the codes of K, those of V and the scales of
+// both (q8.hpp).
 // The block table [seqs * max_pages] u32 lives in its own allocation and is
 // shared by all layers.
 #include <algorithm>
@@ -15,6 +17,7 @@
 #include <string>
 
 #include "pool.hpp"
+#include "q8.hpp"
 
 namespace thb {
 
@@ -364,10 +367,14 @@ int thb_pool_create(const thb_pool_desc* d, thb_pool** out) {
     *out = nullptr;
     if (d->layers == 0) return fail(THB_ERR_CONFIG, "pool needs at least one layer");
     if (d->kv_heads == 0) return fail(THB_ERR_CONFIG, "kv_heads must be positive");
-    if (d->kv_dtype != THB_KV_BF16_TRUNC && d->kv_dtype != THB_KV_F16_RNE)
+    if (d->kv_dtype != THB_KV_BF16_TRUNC && d->kv_dtype != THB_KV_F16_RNE && d->kv_dtype != THB_KV_E4M3)
         return fail(THB_ERR_CONFIG, "unknown kv_dtype " + std::to_string(d->kv_dtype));
     if (d->page_len < 8 || d->page_len > 256 || (d->page_len & (d->page_len - 1)))
         return fail(THB_ERR_CONFIG, "page_len " + std::to_string(d->page_len) + " must be a power of two in [8, 256]");
+    const bool q8 = d->kv_dtype == THB_KV_E4M3;
+    if (q8 && d->page_len < 16)
+        return fail(THB_ERR_CONFIG, "page_len " + std::to_string(d->page_len) +
+                                        " must be at least 16 in an 8-bit pool (tiles of 16 slots)");
     uint32_t part = d->part_len ? d->part_len : 4096;
     // At most 1008 pages: a partition may run part_len / 64 longer (a span a
     // few keys over a multiple of part_len), and the kernels stage at most
@@ -400,8 +407,16 @@ int thb_pool_create(const thb_pool_desc* d, thb_pool** out) {
                 return fail(THB_ERR_CONFIG, "page_len " + std::to_string(d->page_len) + " holds at most 4 GiB per KV-head plane (layer " +
                                                 std::to_string(l) + " needs " + std::to_string(pool_len * hd * 2) +
                                                 " bytes); use page_len >= 16");
+            if (q8) {  // codes of K, codes of V, scales of both (q8.hpp)
+                const uint64_t codes =
+                    (static_cast<uint64_t>(d->kv_heads) * pool_len * q8_width(hd) + 255) & ~uint64_t(255);
+                const uint64_t scales = (static_cast<uint64_t>(d->kv_heads) * pool_len * 2 + 255) & ~uint64_t(255);
+                p->geom.push_back({hd, off, off + codes, off + 2 * codes});
+                off += 2 * codes + scales;
+                continue;
+            }
             uint64_t plane = (static_cast<uint64_t>(d->kv_heads) * pool_len * hd * 2 + 255) & ~uint64_t(255);
-            p->geom.push_back({hd, off, off + plane});
+            p->geom.push_back({hd, off, off + plane, 0});
             off += 2 * plane;
         }
         p->mem_bytes = off;
@@ -433,7 +448,7 @@ int thb_pool_create(const thb_pool_desc* d, thb_pool** out) {
         init_page_state(p.get());
         p->fixed_stager.init(THB_NOALLOC_PLAN_BYTES);
         std::vector<DevLayer> dl;
-        for (const auto& g : p->geom) dl.push_back({g.k_off, g.v_off, g.head_dim, 0});
+        for (const auto& g : p->geom) dl.push_back({g.k_off, g.v_off, g.s_off, g.head_dim, 0});
         void* gd = p->geom_buf.reserve(dl.size() * sizeof(DevLayer), false, nullptr);
         THB_HIP(hipMemcpy(gd, dl.data(), dl.size() * sizeof(DevLayer), hipMemcpyHostToDevice));
         THB_HIP(hipDeviceSynchronize());
@@ -518,8 +533,8 @@ int thb_pool_layer(const thb_pool* pool, uint32_t layer, void** k_dev, void** v_
         info->max_pages = pool->arena.a.max_pages();
         info->page_len = pool->page_len;
         info->kv_dtype = pool->kv_dtype;
-        info->plane_elems = static_cast<uint64_t>(info->pool_len) * g.head_dim;
-        info->page_layout = THB_PAGE_LAYOUT_MFMA;
+        info->plane_elems = static_cast<uint64_t>(info->pool_len) * (is_q8(pool) ? q8_width(g.head_dim) : g.head_dim);
+        info->page_layout = is_q8(pool) ? THB_PAGE_LAYOUT_Q8 : THB_PAGE_LAYOUT_MFMA;
     }
     return THB_OK;
 }

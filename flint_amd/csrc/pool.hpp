@@ -15,6 +15,7 @@ namespace thb {
 // Per-layer record the block-copy kernel reads on the device.
 struct DevLayer {
     uint64_t k_off, v_off;  // byte offsets into the arena
+    uint64_t s_off;         // scales of an 8-bit pool
     uint32_t head_dim, pad;
 };
 
@@ -22,6 +23,7 @@ struct LayerGeom {
     uint32_t head_dim;
     uint64_t k_off;  // byte offsets into the arena
     uint64_t v_off;
+    uint64_t s_off;  // scales (8-bit pools, q8.hpp)
 };
 
 // One cached attention launch plan (see attention.hip).
@@ -129,6 +131,11 @@ struct thb_pool {
     const void* runs_rows = nullptr;
     uint64_t runs_version = ~0ull;
     uint32_t runs_off = 0, runs_m = 0, runs_max = 0, runs_n = 0, runs_long = 0;
+    // Rows of the last append into an 8-bit pool that were found distinct
+    // (checked once per row-meta write, as the model appends them to every layer).
+    const void* distinct_rows = nullptr;
+    uint64_t distinct_version = ~0ull;
+    uint32_t distinct_off = 0, distinct_m = 0;
     std::array<thb::AttnPlan, 4> plans;
     uint64_t plan_clock = 0;
     int device = 0;
@@ -136,6 +143,16 @@ struct thb_pool {
 };
 
 namespace thb {
+inline bool is_q8(const thb_pool* p) { return p->kv_dtype == THB_KV_E4M3; }
+// Append and read-back of 8-bit pools (kv_q8.hip): rows [row_off, row_off + m)
+// of the row meta, checked by the caller.
+void launch_q8_store(thb_pool* p, uint32_t layer, const void* k_src, const void* v_src, uint32_t src_dtype,
+                     const thb_rope* rope, const thb_rows* rows, uint32_t row_off, uint32_t m, hipStream_t s);
+void launch_q8_load(thb_pool* p, uint32_t layer, void* k_dst, void* v_dst, uint32_t dst_dtype, const thb_rows* rows,
+                    uint32_t row_off, uint32_t m, hipStream_t s);
+// Refuses two rows of one token among [row_off, row_off + m): their vectors
+// would be written side by side, and one's codes could meet the other's scale.
+int check_rows_distinct(thb_pool* p, const thb_rows* rows, uint32_t row_off, uint32_t m);
 // Runs the queued page-API calls on the device allocator (and their page
 // copies) before the next kernel on `stream`.  Allocates nothing.
 void pool_flush(thb_pool* p, hipStream_t stream);

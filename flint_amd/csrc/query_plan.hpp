@@ -74,7 +74,7 @@ struct QueryPlan {
 // power of two, then lowered if the aligned part length leaves trailing
 // parts empty): a function of its own key range only.  G: query heads per KV
 // head; PL: part_len; align: a part's length is a multiple of it; WB: query
-// groups per block.
+// groups per block (0: no blocks).
 inline QueryPlan plan_groups(const RowPlan& rp, uint32_t G, uint32_t PL, uint32_t align, uint32_t WB) {
     QueryPlan qp;
     auto& groups = qp.groups;
@@ -121,7 +121,7 @@ inline QueryPlan plan_groups(const RowPlan& rp, uint32_t G, uint32_t PL, uint32_
         }
         const uint32_t ncg = static_cast<uint32_t>(groups.size() / kGroupWords) - first;
         in_block.resize(first + ncg, 0);
-        if (G > kCols || ncg < 4) continue;
+        if (G > kCols || ncg < 4 || WB == 0) continue;
         for (uint32_t b = 0; b < ncg; b += WB) {
             const uint32_t g0 = first + b, ng = std::min(WB, ncg - b);
             uint32_t lo = 0xFFFFFFFFu, hi = 0;

@@ -133,6 +133,20 @@ def kv_store(k_src, v_src, kv: KvPool, layer: int, m: int, meta: RowMeta, row_of
                              meta.handle, row_off, m, _stream_ptr(stream)))
 
 
+def kv_load(k_dst, v_dst, kv: KvPool, layer: int, m: int, meta: RowMeta, row_off: int = 0, stream=None) -> None:
+    """Inverse of kv_store for an "e4m3" pool (no reference counterpart): the
+    stored K and V of the tokens of rows [row_off, row_off+m), as f32, f16 or
+    bf16 [m, kv_heads, head_dim].  Exact in f32 and bf16; storing them again
+    gives the same values."""
+    n = m * kv.kv_heads * _head_dim(kv, layer)
+    _buf("k_dst", k_dst, n, _ACT)
+    _buf("v_dst", v_dst, n, _ACT)
+    if not isinstance(k_dst, int) and not isinstance(v_dst, int) and k_dst.dtype != v_dst.dtype:
+        raise ThubanError(_lib.THB_ERR_INVALID, f"k_dst and v_dst dtypes differ ({k_dst.dtype}, {v_dst.dtype})")
+    check(lib().thb_kv_load(kv.handle, layer, _addr("k_dst", k_dst), _addr("v_dst", v_dst),
+                            _dtype_code(getattr(k_dst, "dtype", None)), meta.handle, row_off, m, _stream_ptr(stream)))
+
+
 def _spec_c(spec: AttnSpec, q, y) -> _lib.AttnSpecC:
     c = _lib.AttnSpecC()
     c.q_heads, c.window, c.scale, c.m = spec.q_heads, spec.window, spec.scale, spec.m
@@ -377,5 +391,5 @@ def block_copy(kv: KvPool, triples: Sequence[Sequence[int]], stream=None) -> Non
 
 
 __all__ = ["AttnSpec", "ThubanError", "attn", "attn_step", "block_copy", "check_gemm_dims", "check_head_dim",
-           "default_scale", "gemm_acc", "kv_gather", "kv_gather_batch", "kv_scatter", "kv_scatter_batch", "kv_store",
-           "kv_store_attn"]
+           "default_scale", "gemm_acc", "kv_gather", "kv_gather_batch", "kv_load", "kv_scatter", "kv_scatter_batch",
+           "kv_store", "kv_store_attn"]

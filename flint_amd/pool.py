@@ -170,12 +170,17 @@ class KvArena:
 
 class KvPool:
     """Device KV of ``layers`` layers sharing one page allocator
-    (KvArena + one KvPool per layer in the reference, model.rs:103-124)."""
+    (KvArena + one KvPool per layer in the reference, model.rs:103-124).
+
+    kv_dtype: "bf16" (truncated, the reference's storage), "f16", or "e4m3":
+    8-bit floats with one power-of-two scale per head vector (THB_KV_E4M3 of
+    include/thuban_hip.h), quantised as they are appended and read back with
+    ``ops.kv_load``."""
 
     def __init__(self, spec: ArenaSpec, kv_heads: int, head_dim: int, layers: int = 1, page_len: int = 32,
                  kv_dtype: str = "bf16", head_dims: Optional[Sequence[int]] = None, part_len: int = 0,
                  arena=None):
-        kv = {"bf16": _lib.KV_BF16_TRUNC, "f16": _lib.KV_F16_RNE}[kv_dtype]
+        kv = {"bf16": _lib.KV_BF16_TRUNC, "f16": _lib.KV_F16_RNE, "e4m3": _lib.KV_E4M3}[kv_dtype]
         d = _lib.PoolDesc()
         d.layers, d.kv_heads, d.head_dim = layers, kv_heads, head_dim
         self._hd_arr = _lib.u32_array(list(head_dims)) if head_dims is not None else None
@@ -280,8 +285,12 @@ class KvPool:
     def layer_tensors(self, layer: int):
         """torch views (16-bit words, no copy) of the layer's device planes as
         stored, one flat page per row: [kv_heads, pages, page_len * head_dim]
-        (the element order inside a page is page_offsets())."""
+        (the element order inside a page is page_offsets()).  16-bit pools
+        only: ops.kv_load reads an 8-bit pool."""
         import torch
+
+        if self.kv_dtype == "e4m3":
+            raise _lib.ThubanError(_lib.THB_ERR_CONFIG, "an 8-bit pool has no 16-bit words: read it with ops.kv_load")
 
         info = self.layer_info(layer)
         k, v = self.layer_ptrs(layer)

@@ -68,6 +68,23 @@ extern "C" {
  * F16_RNE is IEEE half with round-to-nearest-even (thuban_num lib.rs:25-60). */
 #define THB_KV_BF16_TRUNC 0u
 #define THB_KV_F16_RNE 1u
+/* No reference counterpart: 8 bits.  The head vector x of one token and KV head
+ * (K or V) is stored as head_dim codes in e4m3 (4 exponent bits, 3 mantissa
+ * bits, largest value 448) and one power-of-two scale: with e the least integer
+ * for which max|x| <= 448 * 2^e (at least -126), code[d] = x[d] * 2^-e rounded to
+ * the nearest e4m3 value, ties to even, and the stored value is code[d] * 2^e.
+ * A vector that holds an infinity or a NaN is stored as NaN in every element.
+ * Values are exact in f32 and bf16, and storing them again gives the same
+ * values.  In a pool of this type:
+ *  - page_len is at least 16;
+ *  - thb_kv_store, thb_kv_store_rope and the appending attention calls
+ *    quantise as they write, and refuse two rows of one token
+ *    (THB_ERR_INVALID; in a graph's replays the caller sees to it);
+ *  - thb_kv_load reads values back; thb_kv_gather, thb_kv_scatter and their
+ *    batched forms, which move 16-bit words, are refused (THB_ERR_CONFIG);
+ *  - attention, the page API, forks and block copies work as on any pool;
+ *  - device plans are fixed-grid ones without an append (flags 0). */
+#define THB_KV_E4M3 2u
 
 /* Block-table sentinel for a missing page (u32::MAX, pool.rs:85-93). */
 #define THB_NO_PAGE 0xFFFFFFFFu
@@ -155,6 +172,14 @@ int thb_arena_refs(const thb_arena* arena, uint32_t* refs, size_t cap);
  * cache lines.  thb_kv_gather returns both in the reference's token-major
  * layout. */
 #define THB_PAGE_LAYOUT_MFMA 2u
+/* Pages of THB_KV_E4M3 pools: page_len x W one-byte codes (W = head_dim rounded
+ * up to 64), in 1 KiB blocks of 16 slots x 64 dims.  Byte of (slot s, dim d) in
+ * a page, with t = (s / 16) * 16 W + (d / 64) * 1024:
+ *   K: t + (d / 8 % 4) * 256 + (s % 16) * 16 + (d / 32 % 2) * 8 + d % 8
+ *   V: t + (s / 4 % 4) * 256 + (d % 64) * 4 + s % 4
+ * The scales (bytes e + 127; 255 for a vector of NaN) of a layer follow its V
+ * plane, [kv_heads, pages, page_len / 4, 2 (K, V), 4]. */
+#define THB_PAGE_LAYOUT_Q8 3u
 typedef struct thb_pool thb_pool;
 
 typedef struct thb_pool_desc {
@@ -271,6 +296,15 @@ const uint32_t* thb_rows_device(const thb_rows* rows);
  * 16-byte aligned.  Bit-exact: bf16 truncation or f16 RNE as thuban_num. */
 int thb_kv_store(thb_pool* pool, uint32_t layer, const void* k_src_dev, const void* v_src_dev, uint32_t src_dtype,
                  const thb_rows* rows, uint32_t row_off, uint32_t m, void* stream);
+
+/* No reference counterpart: the inverse of thb_kv_store for pools of
+ * THB_KV_E4M3.  The stored K and V of the tokens of rows [row_off, row_off + m)
+ * of the row meta, as dst_dtype (THB_DT_*, rounded to nearest even; exact in f32
+ * and bf16) to dst [m, kv_heads, head_dim], 16-byte aligned.  Rows may repeat a
+ * token.  Captured, it replays as thb_kv_store does; a replayed row whose page
+ * its sequence does not hold leaves its destination as it was. */
+int thb_kv_load(thb_pool* pool, uint32_t layer, void* k_dst_dev, void* v_dst_dev, uint32_t dst_dtype,
+                const thb_rows* rows, uint32_t row_off, uint32_t m, void* stream);
 
 /* ops::AttnSpec (ops/attn.rs:8-16) plus the extensions of this backend. */
 typedef struct thb_attn_spec {
