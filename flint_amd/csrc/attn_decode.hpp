@@ -393,21 +393,29 @@ __device__ inline void store_y(const AttnArgs& a, uint32_t row, uint32_t head, u
     }
 }
 
-// The query elements of a lane: column (row, head), dims 32j + 8 a4 .. + 8 of
-// k-step j, as f32.  In the FULL kernels: query heads q_stride apart and,
-// with rope on, the query head is first normalised (q_norm; the four lanes
-// of the column add their sums of squares) and rotated at the row's
-// position.  Every lane must call it (column sums).
-template <int KS, bool FULL>
+// Hands the query elements of a lane to done(x): column (row, head), dims 32j +
+// 8 a4 .. + 8 of k-step j, as f32.  In the FULL kernels: query heads q_stride
+// apart and, with rope on, the query head is first normalised (q_norm; the four
+// lanes of the column add their sums of squares) and rotated at the row's
+// position.  Every lane must call it (column sums).  (done has a copy in either
+// branch: joined, the kernels of the plain query took up to 10 % longer.)
+template <int KS, bool FULL, class F>
 __device__ __forceinline__ void load_q_f32(const AttnArgs& a, bool con, uint32_t row, uint32_t head, uint32_t a4,
-                                           float (&x)[KS][8]) {
+                                           F&& done) {
     const uint32_t hd = a.head_dim;
     const uint64_t qbase = (static_cast<uint64_t>(row) * a.q_heads + head) * (FULL ? a.q_stride : hd);
-    load_q_all<KS, FULL>(a, con, qbase, a4, x);
-    if (!FULL || !a.rope_on) return;
+    const bool rope = FULL && a.rope_on;
+    if (!rope) {
+        float x[KS][8];
+        load_q_all<KS, FULL>(a, con, qbase, a4, x);
+        done(x);
+        return;
+    }
     // Rotary path: the lane's chunks in registers, normalised in place.
     const RopeDev& r = a.qrope;
     const uint32_t pos = con ? a.meta[8 * row] : 0u;
+    float x[KS][8];
+    load_q_all<KS, FULL>(a, con, qbase, a4, x);
     float inv = 1.0f;
     if (r.w) {
         float ss = 0.0f;
@@ -449,6 +457,7 @@ __device__ __forceinline__ void load_q_f32(const AttnArgs& a, bool con, uint32_t
             }
         }
     }
+    done(x);
 }
 
 // Q^T operand of a lane (load_q_f32's elements), split into high and low
@@ -458,14 +467,14 @@ __device__ __forceinline__ void load_q_f32(const AttnArgs& a, bool con, uint32_t
 template <int KS, class O, bool FULL>
 __device__ inline void load_q(const AttnArgs& a, bool con, uint32_t row, uint32_t head, uint32_t a4,
                               typename O::in8 (&qh)[KS], typename O::in8 (&ql)[KS], float pre = 1.0f) {
-    float x[KS][8];
-    load_q_f32<KS, FULL>(a, con, row, head, a4, x);
+    load_q_f32<KS, FULL>(a, con, row, head, a4, [&](float (&x)[KS][8]) {
 #pragma unroll
-    for (int j = 0; j < KS; j++) {
+        for (int j = 0; j < KS; j++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[j][e] *= pre;
-        O::split8(x[j], qh[j], ql[j]);
-    }
+            for (int e = 0; e < 8; e++) x[j][e] *= pre;
+            O::split8(x[j], qh[j], ql[j]);
+        }
+    });
 }
 
 // The query operand in LDS (head_dim 512 only: QLDS), else nothing.

@@ -64,26 +64,27 @@ __device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8& h, bf16x
 template <int KS, bool QLO, bool FULL>
 __device__ __forceinline__ float load_q_scaled(const AttnArgs& a, bool con, uint32_t row, uint32_t head, uint32_t a4,
                                                f16x8 (&qh)[KS], f16x8 (&ql)[QLO ? KS : 1]) {
-    float x[KS][8];
-    load_q_f32<KS, FULL>(a, con, row, head, a4, x);
-    uint32_t mx = 0u;
+    uint32_t ef = 15u;
+    load_q_f32<KS, FULL>(a, con, row, head, a4, [&](float (&x)[KS][8]) {
+        uint32_t mx = 0u;
 #pragma unroll
-    for (int j = 0; j < KS; j++) mx = max(mx, q8_amax8(x[j]));
-    mx = max(mx, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mx), 16)));
-    mx = max(mx, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mx), 32)));
-    const uint32_t ef = min(max(mx >> 23, 15u), 253u);
-    const float down = __uint_as_float((268u - ef) << 23);
+        for (int j = 0; j < KS; j++) mx = max(mx, q8_amax8(x[j]));
+        mx = max(mx, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mx), 16)));
+        mx = max(mx, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mx), 32)));
+        ef = min(max(mx >> 23, 15u), 253u);
+        const float down = __uint_as_float((268u - ef) << 23);
 #pragma unroll
-    for (int j = 0; j < KS; j++) {
+        for (int j = 0; j < KS; j++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[j][e] *= down;
-        if constexpr (QLO) {
-            Ops<true>::split8_fast(x[j], qh[j], ql[j]);
-        } else {
+            for (int e = 0; e < 8; e++) x[j][e] *= down;
+            if constexpr (QLO) {
+                Ops<true>::split8_fast(x[j], qh[j], ql[j]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) qh[j][e] = static_cast<_Float16>(x[j][e]);
+                for (int e = 0; e < 8; e++) qh[j][e] = static_cast<_Float16>(x[j][e]);
+            }
         }
-    }
+    });
     return __uint_as_float((ef - 14u) << 23);
 }
 
