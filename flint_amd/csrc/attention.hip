@@ -1875,7 +1875,7 @@ void launch_merge(uint32_t hd_t, dim3 grid, const AttnArgs& a, hipStream_t s) {
     }
 }
 
-int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, AttnPlan& plan) {
+int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, bool q_lo, AttnPlan& plan) {
     const Arena& arena = pool->arena.a;
     const uint32_t m = sp.m;
     const uint32_t* args = rows->host.data() + 8 * static_cast<size_t>(sp.row_off);
@@ -1899,8 +1899,8 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
     std::vector<uint32_t> items, bitems;
     const uint32_t PL = pool->part_len;
     const uint32_t hd_t = template_hd(hd);
-    const bool wide = prefill_wide(hd_t);
-    const uint32_t WB = is_q8(pool) ? 0u : block_groups(wide, hd_t);  // query groups per prefill block
+    const bool q8 = is_q8(pool), wide = !q8 && prefill_wide(hd_t);
+    const uint32_t WB = q8 ? 8u * q8_groups(hd_t, q_lo) : block_groups(wide, hd_t);  // query groups per prefill block
     QueryPlan qp = plan_groups(rp, G, PL, std::max<uint32_t>(pool->page_len, 16), WB);
     auto& groups = qp.groups;
     auto& blocks = qp.blocks;
@@ -1915,7 +1915,8 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
     const bool roomy =  // (a split group has a merge record too, a mixed call a launch order)
         4 * (2 * uint64_t(groups.size()) + dec * (kItemWords + 1) + 2ull * m) <= THB_NOALLOC_PLAN_BYTES - (32u << 10);
     // (Beside head_dims above 128 decode items are a launch of their own.)
-    if (wide && roomy && !blocks.empty()) cut_blocks(qp, WB, hd_t > 128 ? 0 : dec, pool->kv_heads, pool->cus);
+    if ((wide || q8) && roomy && !blocks.empty())
+        cut_blocks(qp, WB, q8 || hd_t > 128 ? 0 : dec, pool->kv_heads, pool->cus);
     if (max_parts > kMaxParts)
         return fail(THB_ERR_CONFIG, "key span of " + std::to_string(qp.max_span) + " tokens exceeds " + std::to_string(kMaxParts) + " partitions of " +
                                         std::to_string(PL) + " tokens");
@@ -2164,7 +2165,7 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
         longest = std::max<uint64_t>(longest, work(gr, 5, 6, 8, 9));
         cols = std::max(cols, gr[1] * gr[3]);
     }
-    plan.spread = !is_q8(pool) && n_items > 0 && n_bitems == 0 && spread_head_dim(hd, pool->page_len) &&
+    plan.spread = !q8 && n_items > 0 && n_bitems == 0 && spread_head_dim(hd, pool->page_len) &&
                   spread_rule(hd, cols, n_items, pool->kv_heads, longest, max_parts);
     plan.merge_off = static_cast<uint32_t>(merge_off);
     plan.hd_t = hd_t;
@@ -2181,6 +2182,8 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
     for (size_t b = 0; b < blocks.size(); b += kBlockWords)
         plan.narrow = plan.narrow && blocks[b + 1] <= THB_PREFILL_WAVES;
     plan.mixed = mixed;
+    plan.ncg = 1;
+    for (size_t b = 0; b < blocks.size(); b += kBlockWords) plan.ncg = std::max(plan.ncg, (blocks[b + 1] + 7) / 8);
 
     // The append can run inside the attention launch when no query reads a
     // token that another workgroup appends: the call is causal, every row's
@@ -2204,7 +2207,7 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
         std::sort(seen.begin(), seen.end());
         fuse = std::adjacent_find(seen.begin(), seen.end()) == seen.end();
     }
-    plan.fusable = fuse && !is_q8(pool);
+    plan.fusable = fuse && !q8;
     return THB_OK;
 }
 
@@ -2243,13 +2246,14 @@ void upload_plan(thb_pool* pool, AttnPlan& plan, hipStream_t s) {
 // Finds or builds the launch plan of this call (cached per rows write, call
 // shape and allocator state); with `upload`, its blob is on the device in
 // plan->dev.  Runs inside guarded().
-int get_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, hipStream_t s, bool upload,
-             AttnPlan** out) {
+int get_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, bool rope, hipStream_t s,
+             bool upload, AttnPlan** out) {
+    const bool q_lo = is_q8(pool) && q8_query_lo(sp.q_dtype, rope);  // (decides an 8-bit pool's block size)
     const uint64_t av = pool->arena.a.version();
     for (auto& p : pool->plans)
         if (p.rows == rows && p.rows_version == rows->version && p.arena_version == av && p.row_off == sp.row_off &&
             p.m == sp.m && p.seq == sp.seq && p.causal == sp.causal && p.window == sp.window &&
-            p.q_heads == sp.q_heads && p.head_dim == hd) {
+            p.q_heads == sp.q_heads && p.head_dim == hd && p.q_lo == q_lo) {
             p.last_use = ++pool->plan_clock;
             if (upload) upload_plan(pool, p, s);
             *out = &p;
@@ -2259,7 +2263,7 @@ int get_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint
     for (auto& p : pool->plans)
         if (p.last_use < plan->last_use) plan = &p;
     plan->rows = nullptr;
-    if (int rc = build_plan(pool, rows, sp, hd, *plan)) return rc;
+    if (int rc = build_plan(pool, rows, sp, hd, q_lo, *plan)) return rc;
     if (upload) upload_plan(pool, *plan, s);
     plan->rows = rows;
     plan->rows_version = rows->version;
@@ -2271,6 +2275,7 @@ int get_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint
     plan->window = sp.window;
     plan->q_heads = sp.q_heads;
     plan->head_dim = hd;
+    plan->q_lo = q_lo;
     plan->last_use = ++pool->plan_clock;
     *out = plan;
     return THB_OK;
@@ -2380,6 +2385,8 @@ void launch_plan(thb_pool* pool, uint32_t layer, const thb_attn_io& io, const th
     if (is_q8(pool)) {
         if (n_wg) launch_q8_decode(hd_t, dim3(static_cast<uint32_t>(n_wg)), a, s);
         THB_HIP(hipGetLastError());
+        if (n_pwg) launch_q8_prefill(hd_t, plan.ncg, dim3(static_cast<uint32_t>(n_pwg)), a, s);
+        THB_HIP(hipGetLastError());
     } else if (plan.mixed) {
         launch_mixed(hd_t, f16, plan.narrow, dim3(static_cast<uint32_t>(n_wg + n_pwg)), a, s);
         THB_HIP(hipGetLastError());
@@ -2462,7 +2469,7 @@ int step_impl(thb_pool* pool, uint32_t layer, const thb_attn_io* io, const thb_a
         hipStream_t s = as_stream(stream);
         pool_flush(pool, s);
         AttnPlan* plan = nullptr;
-        if (int rc = get_plan(pool, rows, *spec, hd, s, true, &plan)) return rc;
+        if (int rc = get_plan(pool, rows, *spec, hd, rope != nullptr, s, true, &plan)) return rc;
         const uint32_t* meta = rows->dev + 8 * static_cast<size_t>(spec->row_off);
         const uint32_t* blob = static_cast<const uint32_t*>(plan->dev.get());
         uint64_t o_bytes = 0;
@@ -2601,7 +2608,7 @@ extern "C" int thb_attn_noalloc(thb_pool* pool, uint32_t layer, const void* q, v
         hipStream_t s = as_stream(stream);
         pool_flush(pool, s);  // page ops in kernel arguments, copies from the device list: no allocation
         AttnPlan* plan = nullptr;
-        if (int rc = get_plan(pool, rows, *spec, hd, s, false, &plan)) return rc;
+        if (int rc = get_plan(pool, rows, *spec, hd, false, s, false, &plan)) return rc;
         const uint64_t plan_bytes = plan->blob.size() * 4;
         if (plan_bytes > THB_NOALLOC_PLAN_BYTES)
             return fail(THB_ERR_INVALID, "launch plan of " + std::to_string(plan_bytes) +

@@ -137,6 +137,15 @@ void launch_pick(uint32_t hd, bool f16, dim3 grid, const AttnArgs& a, hipStream_
 // Decode items over an 8-bit pool (attn_q8.hip), one per workgroup; hd is the
 // head_dim template (64, 128, 256 or 512).
 void launch_q8_decode(uint32_t hd, dim3 grid, const AttnArgs& a, hipStream_t s);
+// Prefill blocks over an 8-bit pool, of at most 8 * ncg groups; head_dim <= 256.
+void launch_q8_prefill(uint32_t hd, uint32_t ncg, dim3 grid, const AttnArgs& a, hipStream_t s);
+// Whether the f16 operand of a query needs a low half: an f16 or bf16 query read
+// as it is does not.
+inline bool q8_query_lo(uint32_t q_dt, bool rope) { return q_dt == THB_DT_F32 || rope; }
+// Query groups a wave of attn_q8_prefill can take: what its registers hold.
+constexpr uint32_t q8_groups(uint32_t hd, bool query_lo) {
+    return hd <= 64 ? 3u : hd <= 128 ? (query_lo ? 2u : 3u) : hd <= 256 ? 1u : 0u;
+}
 
 namespace {
 

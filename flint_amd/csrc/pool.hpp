@@ -33,6 +33,7 @@ struct AttnPlan {
     uint64_t rows_version = ~0ull;
     uint64_t arena_version = ~0ull;
     uint32_t row_off = 0, m = 0, seq = 0, causal = 0, window = 0, q_heads = 0, head_dim = 0;
+    bool q_lo = false;  // 8-bit pools: the query has a low half (q8_query_lo)
     // value
     uint32_t n_groups = 0, n_items = 0;     // decode work items
     uint32_t n_blocks = 0, n_bitems = 0;    // prefill blocks and their work items
@@ -41,6 +42,7 @@ struct AttnPlan {
     uint32_t hd_t = 0;   // head_dim template of the kernel
     bool wide = false;   // prefill blocks run attn_prefill_wide (head_dim <= 128)
     bool narrow = false; // no block has more groups than attn_prefill_wide has waves
+    uint32_t ncg = 1;    // 8-bit pools: query groups per wave of the largest prefill block
     bool mixed = false;  // decode items and prefill blocks run as one launch (attn_mixed)
     bool spread = false; // decode items run one wave per workgroup (attn_spread)
     bool split = false;  // some group spans several partitions: merge kernel runs
