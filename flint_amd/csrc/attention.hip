@@ -1875,7 +1875,7 @@ void launch_merge(uint32_t hd_t, dim3 grid, const AttnArgs& a, hipStream_t s) {
     }
 }
 
-int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, bool q_lo, AttnPlan& plan) {
+int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, bool blocks_ok, bool q_lo, AttnPlan& plan) {
     const Arena& arena = pool->arena.a;
     const uint32_t m = sp.m;
     const uint32_t* args = rows->host.data() + 8 * static_cast<size_t>(sp.row_off);
@@ -1900,8 +1900,29 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
     const uint32_t PL = pool->part_len;
     const uint32_t hd_t = template_hd(hd);
     const bool q8 = is_q8(pool), wide = !q8 && prefill_wide(hd_t);
-    const uint32_t WB = q8 ? 8u * q8_groups(hd_t, q_lo) : block_groups(wide, hd_t);  // query groups per prefill block
-    QueryPlan qp = plan_groups(rp, G, PL, std::max<uint32_t>(pool->page_len, 16), WB);
+    const uint32_t WB = q8 ? (blocks_ok && hd_t <= kQ8PrefillHd ? kQ8PrefillWaves : 0u) : block_groups(wide, hd_t);  // query groups per prefill block
+    const uint32_t align = std::max<uint32_t>(pool->page_len, 16);
+    QueryPlan qp = plan_groups(rp, G, PL, align, WB);
+    if (q8 && WB) {
+        // Over an 8-bit pool blocks pay from one workgroup per CU on; with fewer their
+        // groups run on the decode kernel, which converts the codes itself but puts each
+        // group on a workgroup of 8 waves (8 KV heads of 128 x 4, us as decode items /
+        // blocks: 512 fresh rows 24.9 / 23.8, 768 39.8 / 31.2, 1024 58.7 / 39.0, 256
+        // after 16000 keys 240 / 165; 32 after 8000 keys 40 / 95).  head_dim 256 stays
+        // there (8 x 2 x 256, 1000 rows after 3000 keys 154 / 210).  From two rounds of
+        // workgroups on, two groups a wave (4096 rows 210 -> 191, 8192 854 -> 779, but
+        // 2048 73 -> 86): not beside a query's low halves, whose registers they would take.
+        auto wgs = [&](const QueryPlan& q) {
+            uint64_t n = 0;
+            for (size_t b = 0; b < q.blocks.size(); b += kBlockWords) n += q.blocks[b + 5];
+            return n * pool->kv_heads;
+        };
+        const uint64_t n = wgs(qp);
+        if (n < pool->cus)
+            qp = plan_groups(rp, G, PL, align, 0);
+        else if (n >= 8ull * pool->cus && hd_t == 128 && !q_lo)
+            qp = plan_groups(rp, G, PL, align, 2 * WB);
+    }
     auto& groups = qp.groups;
     auto& blocks = qp.blocks;
     const auto& in_block = qp.in_block;
@@ -1915,8 +1936,8 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
     const bool roomy =  // (a split group has a merge record too, a mixed call a launch order)
         4 * (2 * uint64_t(groups.size()) + dec * (kItemWords + 1) + 2ull * m) <= THB_NOALLOC_PLAN_BYTES - (32u << 10);
     // (Beside head_dims above 128 decode items are a launch of their own.)
-    if ((wide || q8) && roomy && !blocks.empty())
-        cut_blocks(qp, WB, q8 || hd_t > 128 ? 0 : dec, pool->kv_heads, pool->cus);
+    if (wide && roomy && !blocks.empty())
+        cut_blocks(qp, WB, hd_t > 128 ? 0 : dec, pool->kv_heads, pool->cus);
     if (max_parts > kMaxParts)
         return fail(THB_ERR_CONFIG, "key span of " + std::to_string(qp.max_span) + " tokens exceeds " + std::to_string(kMaxParts) + " partitions of " +
                                         std::to_string(PL) + " tokens");
@@ -2147,6 +2168,28 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
             }
         }
     const uint32_t n_merge = static_cast<uint32_t>((blob.size() - merge_off) / kMergeWords);
+    // An 8-bit pool's key regions: by sequence, all keys that its blocks read.
+    plan.regions_off = blob.size();
+    plan.n_regions = plan.q8_steps = 0;
+    if (q8 && n_blocks) {
+        std::map<uint32_t, std::array<uint32_t, 3>> regions;  // seq -> first key, end, first step
+        for (size_t b = 0; b < blocks.size(); b += kBlockWords) {
+            if (blocks[b + 4] <= blocks[b + 3]) continue;
+            auto it = regions.insert({blocks[b + 2], {blocks[b + 3], blocks[b + 4], 0u}}).first;
+            it->second[0] = std::min(it->second[0], blocks[b + 3]);
+            it->second[1] = std::max(it->second[1], blocks[b + 4]);
+        }
+        for (auto& r : regions) {
+            r.second[2] = plan.q8_steps;
+            plan.q8_steps += static_cast<uint32_t>((uint64_t(r.second[1]) + 31) / 32 - r.second[0] / 32);
+            blob.insert(blob.end(), {r.first, r.second[0], r.second[1], r.second[2]});
+        }
+        plan.n_regions = static_cast<uint32_t>(regions.size());
+        for (uint32_t i = 0; i < n_bitems; i++) {
+            const auto it = regions.find(blocks[static_cast<size_t>(bitems[i]) * kBlockWords + 2]);
+            blob.push_back(it == regions.end() ? 0u : it->second[2] - it->second[0] / 32);
+        }
+    }
     plan.blob.swap(blob);
     plan.uploaded = false;
     plan.n_groups = n_groups;
@@ -2183,7 +2226,8 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
         plan.narrow = plan.narrow && blocks[b + 1] <= THB_PREFILL_WAVES;
     plan.mixed = mixed;
     plan.ncg = 1;
-    for (size_t b = 0; b < blocks.size(); b += kBlockWords) plan.ncg = std::max(plan.ncg, (blocks[b + 1] + 7) / 8);
+    for (size_t b = 0; b < blocks.size(); b += kBlockWords) 
+        plan.ncg = std::max(plan.ncg, (blocks[b + 1] + kQ8PrefillWaves - 1) / kQ8PrefillWaves);
 
     // The append can run inside the attention launch when no query reads a
     // token that another workgroup appends: the call is causal, every row's
@@ -2248,12 +2292,14 @@ void upload_plan(thb_pool* pool, AttnPlan& plan, hipStream_t s) {
 // plan->dev.  Runs inside guarded().
 int get_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, bool rope, hipStream_t s,
              bool upload, AttnPlan** out) {
-    const bool q_lo = is_q8(pool) && q8_query_lo(sp.q_dtype, rope);  // (decides an 8-bit pool's block size)
+    // An 8-bit pool's prefill blocks: their size depends on the query's halves, and the
+    // no-allocation call has no scratch for their expanded keys.
+    const bool q_lo = is_q8(pool) && q8_query_lo(sp.q_dtype, rope), blocks_ok = !is_q8(pool) || upload;
     const uint64_t av = pool->arena.a.version();
     for (auto& p : pool->plans)
         if (p.rows == rows && p.rows_version == rows->version && p.arena_version == av && p.row_off == sp.row_off &&
             p.m == sp.m && p.seq == sp.seq && p.causal == sp.causal && p.window == sp.window &&
-            p.q_heads == sp.q_heads && p.head_dim == hd && p.q_lo == q_lo) {
+            p.q_heads == sp.q_heads && p.head_dim == hd && p.q_lo == q_lo && p.blocks_ok == blocks_ok) {
             p.last_use = ++pool->plan_clock;
             if (upload) upload_plan(pool, p, s);
             *out = &p;
@@ -2263,7 +2309,7 @@ int get_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint
     for (auto& p : pool->plans)
         if (p.last_use < plan->last_use) plan = &p;
     plan->rows = nullptr;
-    if (int rc = build_plan(pool, rows, sp, hd, q_lo, *plan)) return rc;
+    if (int rc = build_plan(pool, rows, sp, hd, blocks_ok, q_lo, *plan)) return rc;
     if (upload) upload_plan(pool, *plan, s);
     plan->rows = rows;
     plan->rows_version = rows->version;
@@ -2276,6 +2322,7 @@ int get_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint
     plan->q_heads = sp.q_heads;
     plan->head_dim = hd;
     plan->q_lo = q_lo;
+    plan->blocks_ok = blocks_ok;
     plan->last_use = ++pool->plan_clock;
     *out = plan;
     return THB_OK;
@@ -2293,6 +2340,11 @@ uint64_t partial_bytes(const thb_pool* pool, const AttnPlan& plan, bool spread, 
     const uint64_t n_part = static_cast<uint64_t>(plan.n_slots) * per * pool->kv_heads * kCols;
     *o_bytes = (n_part * plan.hd_t * 4 + 255) & ~uint64_t(255);
     return *o_bytes + n_part * 8;
+}
+
+// Bytes of an 8-bit pool's expanded keys (a multiple of 256).
+uint64_t expanded_bytes(const thb_pool* pool, const AttnPlan& plan) {
+    return (plan.q8_steps * q8_step_bytes(plan.hd_t) * pool->kv_heads + 255) & ~uint64_t(255);
 }
 
 // The arguments of every attention launch that do not depend on the plan's
@@ -2345,8 +2397,8 @@ void fill_args(thb_pool* pool, uint32_t layer, const thb_attn_io& io, const thb_
 // loaded (and the fused append rotates the key); meta is the row meta of
 // the call's first row.
 void launch_plan(thb_pool* pool, uint32_t layer, const thb_attn_io& io, const thb_attn_spec& sp, const AttnPlan& plan,
-                 bool fused_append, const uint32_t* meta, const uint32_t* blob, uint8_t* part, uint32_t* merge_cnt,
-                 hipStream_t s) {
+                 bool fused_append, const uint32_t* meta, const uint32_t* blob, uint8_t* part, uint8_t* expanded,
+                 uint32_t* merge_cnt, hipStream_t s) {
     const uint32_t hd_t = plan.hd_t;
     float* part_o = nullptr;
     float* part_ml = nullptr;
@@ -2385,6 +2437,15 @@ void launch_plan(thb_pool* pool, uint32_t layer, const thb_attn_io& io, const th
     if (is_q8(pool)) {
         if (n_wg) launch_q8_decode(hd_t, dim3(static_cast<uint32_t>(n_wg)), a, s);
         THB_HIP(hipGetLastError());
+        if (plan.q8_steps) {
+            a.regions = blob + plan.regions_off;
+            a.bregions = a.regions + static_cast<size_t>(plan.n_regions) * kQ8RegionWords;
+            a.n_regions = plan.n_regions;
+            a.steps = plan.q8_steps;
+            a.expanded = expanded;
+            launch_q8_expand(hd_t, a, s);
+            THB_HIP(hipGetLastError());
+        }
         if (n_pwg) launch_q8_prefill(hd_t, plan.ncg, dim3(static_cast<uint32_t>(n_pwg)), a, s);
         THB_HIP(hipGetLastError());
     } else if (plan.mixed) {
@@ -2474,12 +2535,14 @@ int step_impl(thb_pool* pool, uint32_t layer, const thb_attn_io* io, const thb_a
         const uint32_t* blob = static_cast<const uint32_t*>(plan->dev.get());
         uint64_t o_bytes = 0;
         const uint64_t pb = partial_bytes(pool, *plan, plan->spread, &o_bytes);
-        uint8_t* part = pb ? static_cast<uint8_t*>(pool->partials.reserve(pb, false, s)) : nullptr;
+        const uint64_t xb = expanded_bytes(pool, *plan);  // (first: partial results need 8-byte alignment only)
+        uint8_t* xp = pb + xb ? static_cast<uint8_t*>(pool->partials.reserve(xb + pb, false, s)) : nullptr;
+        uint8_t* part = xp + xb;
         uint32_t* cnt = plan->n_merge_dec || plan->spread ? static_cast<uint32_t*>(pool->merge_cnt.reserve(
                                                 static_cast<size_t>(plan->n_items) * pool->kv_heads * 4, true, s))
                                           : nullptr;
         if (!append) {
-            launch_plan(pool, layer, *io, *spec, *plan, false, meta, blob, part, cnt, s);
+            launch_plan(pool, layer, *io, *spec, *plan, false, meta, blob, part, xp, cnt, s);
             return THB_OK;
         }
         // The row meta's sequence must be the one the append uses: a fixed
@@ -2489,7 +2552,7 @@ int step_impl(thb_pool* pool, uint32_t layer, const thb_attn_io* io, const thb_a
             for (uint32_t r = spec->row_off; r < spec->row_off + spec->m && fuse; r++)
                 fuse = rows->host[8 * r + 1] == spec->seq;
         if (fuse) {
-            launch_plan(pool, layer, *io, *spec, *plan, true, meta, blob, part, cnt, s);
+            launch_plan(pool, layer, *io, *spec, *plan, true, meta, blob, part, xp, cnt, s);
             return THB_OK;
         }
         const int rc = rope ? thb_kv_store_rope(pool, layer, io->k_src_dev, io->v_src_dev, io->src_dtype, rope, rows,
@@ -2497,7 +2560,7 @@ int step_impl(thb_pool* pool, uint32_t layer, const thb_attn_io* io, const thb_a
                             : thb_kv_store(pool, layer, io->k_src_dev, io->v_src_dev, io->src_dtype, rows,
                                            spec->row_off, spec->m, stream);
         if (rc) return rc;
-        launch_plan(pool, layer, *io, *spec, *plan, false, meta, blob, part, cnt, s);
+        launch_plan(pool, layer, *io, *spec, *plan, false, meta, blob, part, xp, cnt, s);
         return THB_OK;
     });
 }
@@ -2625,7 +2688,7 @@ extern "C" int thb_attn_noalloc(thb_pool* pool, uint32_t layer, const void* q, v
         const thb_attn_io io = make_io(q, y, nullptr, nullptr, 0, nullptr);
         const uint32_t* meta = rows->dev + 8 * static_cast<size_t>(spec->row_off);
         launch_plan(pool, layer, io, *spec, *plan, false, meta, reinterpret_cast<const uint32_t*>(scr),
-                    scr + THB_NOALLOC_PLAN_BYTES, nullptr, s);
+                    scr + THB_NOALLOC_PLAN_BYTES, nullptr, nullptr, s);
         return THB_OK;
     });
 }

@@ -127,6 +127,13 @@ struct AttnArgs {
     const uint32_t* meta;  // row meta of the call's rows (positions)
     RopeDev qrope, krope;
     uint8_t* scales;  // an 8-bit pool's scales (q8.hpp); k and v then address its codes
+    // An 8-bit pool's prefill blocks: their key regions (sequence, first key, end,
+    // first step in the scratch: kQ8RegionWords each), by work item the scratch's
+    // step of key 0 (modulo 2^32), and the scratch, of `steps` steps a KV head.
+    const uint32_t* regions;
+    const uint32_t* bregions;
+    uint8_t* expanded;
+    uint32_t n_regions, steps;
 };
 
 // Decode items one wave per workgroup (attn_spread.hip; head_dim 64, 128 or
@@ -137,15 +144,19 @@ void launch_pick(uint32_t hd, bool f16, dim3 grid, const AttnArgs& a, hipStream_
 // Decode items over an 8-bit pool (attn_q8.hip), one per workgroup; hd is the
 // head_dim template (64, 128, 256 or 512).
 void launch_q8_decode(uint32_t hd, dim3 grid, const AttnArgs& a, hipStream_t s);
-// Prefill blocks over an 8-bit pool, of at most 8 * ncg groups; head_dim <= 256.
+// Prefill blocks over an 8-bit pool, of at most kQ8PrefillWaves * ncg groups (ncg 2 only
+// at head_dim 128 and a query without a low half), behind the expansion of their keys.
+void launch_q8_expand(uint32_t hd, const AttnArgs& a, hipStream_t s);
 void launch_q8_prefill(uint32_t hd, uint32_t ncg, dim3 grid, const AttnArgs& a, hipStream_t s);
 // Whether the f16 operand of a query needs a low half: an f16 or bf16 query read
 // as it is does not.
 inline bool q8_query_lo(uint32_t q_dt, bool rope) { return q_dt == THB_DT_F32 || rope; }
-// Query groups a wave of attn_q8_prefill can take: what its registers hold.
-constexpr uint32_t q8_groups(uint32_t hd, bool query_lo) {
-    return hd <= 64 ? 3u : hd <= 128 ? (query_lo ? 2u : 3u) : hd <= 256 ? 1u : 0u;
-}
+constexpr uint32_t kQ8PrefillWaves = 4;
+constexpr uint32_t kQ8PrefillHd = 128;  // the largest head_dim that has prefill blocks
+// Scratch of a call's prefill blocks: per KV head and step of 32 keys the expanded
+// codes and a Q8Ref (attn_q8.hip).
+constexpr uint32_t kQ8RefBytes = 32, kQ8RegionWords = 4;
+constexpr uint64_t q8_step_bytes(uint32_t hd_t) { return 128ull * hd_t + kQ8RefBytes; }
 
 namespace {
 

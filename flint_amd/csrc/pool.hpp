@@ -33,7 +33,7 @@ struct AttnPlan {
     uint64_t rows_version = ~0ull;
     uint64_t arena_version = ~0ull;
     uint32_t row_off = 0, m = 0, seq = 0, causal = 0, window = 0, q_heads = 0, head_dim = 0;
-    bool q_lo = false;  // 8-bit pools: the query has a low half (q8_query_lo)
+    bool q_lo = false, blocks_ok = true;  // 8-bit pools: the query has a low half, blocks may be made
     // value
     uint32_t n_groups = 0, n_items = 0;     // decode work items
     uint32_t n_blocks = 0, n_bitems = 0;    // prefill blocks and their work items
@@ -43,13 +43,15 @@ struct AttnPlan {
     bool wide = false;   // prefill blocks run attn_prefill_wide (head_dim <= 128)
     bool narrow = false; // no block has more groups than attn_prefill_wide has waves
     uint32_t ncg = 1;    // 8-bit pools: query groups per wave of the largest prefill block
+    uint32_t n_regions = 0, q8_steps = 0;  // 8-bit pools: key regions of the prefill blocks, steps they expand to
+    size_t regions_off = 0;                // blob offset (words) of the regions, then of each work item's first step
     bool mixed = false;  // decode items and prefill blocks run as one launch (attn_mixed)
     bool spread = false; // decode items run one wave per workgroup (attn_spread)
     bool split = false;  // some group spans several partitions: merge kernel runs
     uint32_t n_merge = 0, merge_off = 0;  // groups of several partitions: count, blob offset (words)
     uint32_t n_merge_dec = 0;             // of those, decode groups (listed first)
     bool fusable = false;  // an append of the call's rows can run inside the launch
-    std::vector<uint32_t> blob;  // [groups | items | row ranges | prefill items | pairs | order | merge list]
+    std::vector<uint32_t> blob;  // [groups | items | row ranges | prefill items | pairs | order | merge list | regions]
     DevBuf dev;                  // blob on the device, when uploaded
     bool uploaded = false;
     uint64_t last_use = 0;
