@@ -322,7 +322,7 @@ __global__ __launch_bounds__(64 * W) void attn_q8(AttnArgs a) {
 // probabilities.  So a score costs no multiply for either scale.  Probabilities
 // are 2^kPBias times too large throughout, which keeps them clear of f16's
 // subnormals (at most 2^(kPBias + kTau) = 2^15), and are one f16 operand for a
-// 16-bit output (2^-12 of each, below the output's own rounding) or split into
+// 16-bit output (each off by at most 2^-11 of itself, an f16 output's own rounding) or split into
 // two for f32 (PLO).  The sum l is taken from the unrounded ones.
 constexpr float kPBias = 7.0f;
 constexpr uint32_t kQ8Up = 7;

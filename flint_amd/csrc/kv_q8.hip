@@ -1,9 +1,9 @@
 // Append (quantise) and read-back kernels of 8-bit pools (THB_KV_E4M3; format
 // and page layout in q8.hpp).
 //
-// Both move head vectors: one lane owns 8 consecutive dims of one vector, the
-// lanes of a vector form a segment (a power of two >= head_dim / 8, at least
-// 8), and a wavefront holds 64 / segment vectors.
+// Both move head vectors: one lane owns 8 consecutive dims of one vector (or of 4,
+// of consecutive rows), the lanes of a vector form a segment (a power of two >=
+// head_dim / 8, at least 8), and a wavefront holds 64 / segment of them.
 #include <algorithm>
 #include <string>
 
@@ -71,42 +71,132 @@ __device__ inline uint32_t q8_seg_max(uint32_t m, uint32_t seg_shift) {
     return m;
 }
 
-template <uint32_t SRC>
+// Rows of a segment: RB consecutive ones of one head.  Groups of RB rows start
+// where the first row's slot would be a multiple of RB, so that those of a chunk
+// of consecutive tokens cover whole groups of RB slots.
+template <uint32_t RB>
+struct Q8Rows {
+    uint32_t u, h, row0;          // the lane's unit of 8 dims, head, first row (may be "negative")
+    uint32_t on, held;            // bits: rows of the call; of those, rows whose page is the pool's
+    uint32_t pos[RB], page[RB];
+    bool run;                     // RB whole rows, at RB consecutive slots from a multiple of RB
+
+    __device__ Q8Rows(const Q8Geom& g, uint32_t bid) {
+        const uint32_t lane = threadIdx.x & 63u;
+        u = lane & ((1u << g.seg_shift) - 1u);
+        const uint32_t i = (bid * 4 + (threadIdx.x >> 6)) * (64u >> g.seg_shift) + (lane >> g.seg_shift);
+        const uint32_t gr = i / g.kv_heads;
+        h = i - gr * g.kv_heads;
+        row0 = gr * RB - (RB > 1 ? g.meta[0] & (RB - 1u) : 0u);
+        on = held = 0;
+        run = RB > 1;
+#pragma unroll
+        for (uint32_t r = 0; r < RB; r++) {
+            pos[r] = page[r] = 0;
+            if (row0 + r < g.m) {  // (a row before the first is a large number)
+                on |= 1u << r;
+                held |= q8_row_page(g, row0 + r, pos[r], page[r]) ? 1u << r : 0u;
+            }
+            run = run && pos[r] == (pos[0] | r) && page[r] == page[0];
+        }
+        run = run && held == (1u << RB) - 1u && (pos[0] & (RB - 1u)) == 0;
+    }
+};
+
+// RB: rows a lane handles.  A byte of V per slot and dim is a store of its own
+// where a token comes alone; RB = 4 tokens of consecutive slots fill the words of
+// their 4-slot groups: 16-byte stores of V, and of K between two lanes that
+// hold the two halves of a slot's 16 bytes.  Bound by its bytes: 4096 bf16 rows of
+// 8 KV heads of 128, 25 MB, 10.1 us, reading them back 9.2; the pair of calls 30,
+// which is their host time (with byte stores 35).
+template <uint32_t SRC, uint32_t RB>
 __global__ __launch_bounds__(256) void q8_store_kernel(Q8StoreArgs a) {
     const Q8Geom& g = a.g;
     const bool is_v = blockIdx.x >= a.k_wgs;
-    const uint32_t bid = is_v ? blockIdx.x - a.k_wgs : blockIdx.x;
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t seg = lane >> g.seg_shift, u = lane & ((1u << g.seg_shift) - 1u);
-    const uint32_t vec = (bid * 4 + (threadIdx.x >> 6)) * (64u >> g.seg_shift) + seg;
-    const uint32_t cph = g.head_dim >> 3;
-    const bool act = vec < g.m * g.kv_heads && u < cph;
-    const uint32_t row = act ? vec / g.kv_heads : 0u, h = act ? vec - row * g.kv_heads : 0u;
-    uint32_t pos = 0, page = 0;
-    const bool held = act && q8_row_page(g, row, pos, page);
-    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (act) q8_load8<SRC>(is_v ? a.v_src : a.k_src, static_cast<uint64_t>(vec) * g.head_dim + 8u * u, x);
-    if (!is_v && a.rope_on) {  // the rotated key is rounded to the source type first, as thb_rope_rows would leave it
-        rope_head_seg(x, act ? u : cph, cph, seg << g.seg_shift, pos, a.rope);
-        if constexpr (SRC == THB_DT_F16) {
+    const Q8Rows<RB> R(g, is_v ? blockIdx.x - a.k_wgs : blockIdx.x);
+    const uint32_t u = R.u, cph = g.head_dim >> 3;
+    float x[RB][8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = __uint_as_float(f16_to_f32_bits(f32_to_f16_rne(x[e])));
+    for (uint32_t r = 0; r < RB; r++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[r][e] = 0.0f;
+        if ((R.on >> r & 1u) && u < cph)
+            q8_load8<SRC>(is_v ? a.v_src : a.k_src,
+                          (static_cast<uint64_t>(R.row0 + r) * g.kv_heads + R.h) * g.head_dim + 8u * u, x[r]);
+    }
+    uint2 w[RB];
+    uint32_t b[RB];
+#pragma unroll
+    for (uint32_t r = 0; r < RB; r++) {
+        if (!is_v && a.rope_on) {  // the rotated key is rounded to the source type first, as thb_rope_rows would leave it
+            rope_head_seg(x[r], (R.on >> r & 1u) && u < cph ? u : cph, cph, (threadIdx.x & 63u) - u, R.pos[r], a.rope);
+            if constexpr (SRC == THB_DT_F16) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[r][e] = __uint_as_float(f16_to_f32_bits(f32_to_f16_rne(x[r][e])));
+            }
+        }
+        b[r] = q8_scale_byte(q8_seg_max(q8_amax8(x[r]), g.seg_shift));
+        w[r] = q8_encode8(x[r], b[r]);
+    }
+    if constexpr (RB == 4) {
+        if (R.run) {
+            const uint32_t j = R.pos[0] & ((1u << g.page_shift) - 1u);
+            const uint64_t pi = q8_page_index(g, R.h, R.page[0]);
+            const uint64_t codes = (pi << g.page_shift) * g.width;
+            if (u == 0)
+                *reinterpret_cast<uint32_t*>(g.s + (pi << g.page_shift) * 2u + q8_s_off(j, is_v)) =
+                    b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+            if (is_v) {
+                if (u >= cph) return;
+                u32x4 t[2];  // by dim, the 4 slots' codes
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    const uint32_t w0 = d ? w[0].y : w[0].x, w1 = d ? w[1].y : w[1].x;
+                    const uint32_t w2 = d ? w[2].y : w[2].x, w3 = d ? w[3].y : w[3].x;
+                    const uint32_t a01 = __builtin_amdgcn_perm(w1, w0, 0x05010400), b01 = __builtin_amdgcn_perm(w1, w0, 0x07030602);
+                    const uint32_t a23 = __builtin_amdgcn_perm(w3, w2, 0x05010400), b23 = __builtin_amdgcn_perm(w3, w2, 0x07030602);
+                    t[d] = u32x4{__builtin_amdgcn_perm(a23, a01, 0x05040100), __builtin_amdgcn_perm(a23, a01, 0x07060302),
+                                 __builtin_amdgcn_perm(b23, b01, 0x05040100), __builtin_amdgcn_perm(b23, b01, 0x07060302)};
+                }
+                u32x4* dst = reinterpret_cast<u32x4*>(g.v + codes + q8_v_off(j, 8u * u, g.width));
+                dst[0] = t[0];
+                dst[1] = t[1];
+                return;
+            }
+            // Units u and u + 4 of a 64-dim block hold a slot's 16 bytes: the first lane
+            // takes rows 0 and 1, the second 2 and 3.  (A block's padding, where
+            // head_dim ends inside it, gets the zero codes it has.)
+            const bool hi = (u & 4u) != 0;
+            u32x4 o[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const uint2 give = hi ? w[r] : w[r + 2], own = hi ? w[r + 2] : w[r];
+                const uint2 got = make_uint2(__shfl_xor(static_cast<int>(give.x), 4), __shfl_xor(static_cast<int>(give.y), 4));
+                o[r] = hi ? u32x4{got.x, got.y, own.x, own.y} : u32x4{own.x, own.y, got.x, got.y};
+            }
+            if (8u * u >= g.width) return;
+            u32x4* dst = reinterpret_cast<u32x4*>(g.k + codes + q8_k_off(j + (hi ? 2u : 0u), 8u * (u & ~4u), g.width));
+            dst[0] = o[0];
+            dst[1] = o[1];
+            return;
         }
     }
-    const uint32_t b = q8_scale_byte(q8_seg_max(q8_amax8(x), g.seg_shift));
-    if (!held) return;
-    const uint2 w = q8_encode8(x, b);
-    const uint32_t j = pos & ((1u << g.page_shift) - 1u);
-    const uint64_t pi = q8_page_index(g, h, page);
-    const uint64_t codes = (pi << g.page_shift) * g.width;
-    if (!is_v) {
-        *reinterpret_cast<uint2*>(g.k + codes + q8_k_off(j, 8u * u, g.width)) = w;
-    } else {
-        uint8_t* dst = g.v + codes + q8_v_off(j, 8u * u, g.width);
+    if (u >= cph) return;
 #pragma unroll
-        for (int e = 0; e < 8; e++) dst[4 * e] = static_cast<uint8_t>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+    for (uint32_t r = 0; r < RB; r++) {
+        if (!(R.held >> r & 1u)) continue;
+        const uint32_t j = R.pos[r] & ((1u << g.page_shift) - 1u);
+        const uint64_t pi = q8_page_index(g, R.h, R.page[r]);
+        const uint64_t codes = (pi << g.page_shift) * g.width;
+        if (!is_v) {
+            *reinterpret_cast<uint2*>(g.k + codes + q8_k_off(j, 8u * u, g.width)) = w[r];
+        } else {
+            uint8_t* dst = g.v + codes + q8_v_off(j, 8u * u, g.width);
+#pragma unroll
+            for (int e = 0; e < 8; e++) dst[4 * e] = static_cast<uint8_t>((e < 4 ? w[r].x : w[r].y) >> (8 * (e & 3)));
+        }
+        if (u == 0) g.s[(pi << g.page_shift) * 2u + q8_s_off(j, is_v)] = static_cast<uint8_t>(b[r]);
     }
-    if (u == 0) g.s[(pi << g.page_shift) * 2u + q8_s_off(j, is_v)] = static_cast<uint8_t>(b);
 }
 
 struct Q8LoadArgs {
@@ -116,37 +206,66 @@ struct Q8LoadArgs {
     uint32_t k_wgs;
 };
 
-template <uint32_t DT>
+template <uint32_t DT, uint32_t RB>
 __global__ __launch_bounds__(256) void q8_load_kernel(Q8LoadArgs a) {
     const Q8Geom& g = a.g;
     const bool is_v = blockIdx.x >= a.k_wgs;
-    const uint32_t bid = is_v ? blockIdx.x - a.k_wgs : blockIdx.x;
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t seg = lane >> g.seg_shift, u = lane & ((1u << g.seg_shift) - 1u);
-    const uint32_t vec = (bid * 4 + (threadIdx.x >> 6)) * (64u >> g.seg_shift) + seg;
-    if (vec >= g.m * g.kv_heads || 8u * u >= g.head_dim) return;
-    const uint32_t row = vec / g.kv_heads, h = vec - row * g.kv_heads;
-    uint32_t pos, page;
-    if (!q8_row_page(g, row, pos, page)) return;
-    const uint32_t j = pos & ((1u << g.page_shift) - 1u);
-    const uint64_t pi = q8_page_index(g, h, page);
-    const uint64_t codes = (pi << g.page_shift) * g.width;
-    const float scale = __uint_as_float(static_cast<uint32_t>(g.s[(pi << g.page_shift) * 2u + q8_s_off(j, is_v)]) << 23);
-    uint2 w;
-    if (!is_v) {
-        w = *reinterpret_cast<const uint2*>(g.k + codes + q8_k_off(j, 8u * u, g.width));
-    } else {
-        const uint8_t* src = g.v + codes + q8_v_off(j, 8u * u, g.width);
-        w = make_uint2(0u, 0u);
+    const Q8Rows<RB> R(g, is_v ? blockIdx.x - a.k_wgs : blockIdx.x);
+    const uint32_t u = R.u;
+    if (8u * u >= g.head_dim) return;
+    uint2 w[RB];
+    uint32_t b[RB];
+    bool run = false;
+    if constexpr (RB == 4) run = R.run && is_v;
+    if (run) {  // the 4-slot words of V, transposed
+        if constexpr (RB == 4) {
+            const uint32_t j = R.pos[0] & ((1u << g.page_shift) - 1u);
+            const uint64_t pi = q8_page_index(g, R.h, R.page[0]);
+            const u32x4* src = reinterpret_cast<const u32x4*>(g.v + (pi << g.page_shift) * g.width + q8_v_off(j, 8u * u, g.width));
+            const uint32_t sw = *reinterpret_cast<const uint32_t*>(g.s + (pi << g.page_shift) * 2u + q8_s_off(j, true));
+            const u32x4 t[2] = {src[0], src[1]};
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            w.x |= static_cast<uint32_t>(src[4 * e]) << (8 * e);
-            w.y |= static_cast<uint32_t>(src[16 + 4 * e]) << (8 * e);
+            for (int r = 0; r < 4; r++) b[r] = sw >> (8 * r) & 255u;
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                const uint32_t a01 = __builtin_amdgcn_perm(t[d][1], t[d][0], 0x05010400), b01 = __builtin_amdgcn_perm(t[d][1], t[d][0], 0x07030602);
+                const uint32_t a23 = __builtin_amdgcn_perm(t[d][3], t[d][2], 0x05010400), b23 = __builtin_amdgcn_perm(t[d][3], t[d][2], 0x07030602);
+                const uint32_t o[4] = {__builtin_amdgcn_perm(a23, a01, 0x05040100), __builtin_amdgcn_perm(a23, a01, 0x07060302),
+                                       __builtin_amdgcn_perm(b23, b01, 0x05040100), __builtin_amdgcn_perm(b23, b01, 0x07060302)};
+#pragma unroll
+                for (int r = 0; r < 4; r++) (d ? w[r].y : w[r].x) = o[r];
+            }
+        }
+    } else {
+#pragma unroll
+        for (uint32_t r = 0; r < RB; r++) {
+            w[r] = make_uint2(0u, 0u);
+            b[r] = 1u;
+            if (!(R.held >> r & 1u)) continue;
+            const uint32_t j = R.pos[r] & ((1u << g.page_shift) - 1u);
+            const uint64_t pi = q8_page_index(g, R.h, R.page[r]);
+            const uint64_t codes = (pi << g.page_shift) * g.width;
+            b[r] = g.s[(pi << g.page_shift) * 2u + q8_s_off(j, is_v)];
+            if (!is_v) {
+                w[r] = *reinterpret_cast<const uint2*>(g.k + codes + q8_k_off(j, 8u * u, g.width));
+            } else {
+                const uint8_t* src = g.v + codes + q8_v_off(j, 8u * u, g.width);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    w[r].x |= static_cast<uint32_t>(src[4 * e]) << (8 * e);
+                    w[r].y |= static_cast<uint32_t>(src[16 + 4 * e]) << (8 * e);
+                }
+            }
         }
     }
-    float x[8];
-    q8_decode8(w, scale, x);
-    q8_put8<DT>(is_v ? a.v_dst : a.k_dst, static_cast<uint64_t>(vec) * g.head_dim + 8u * u, x);
+#pragma unroll
+    for (uint32_t r = 0; r < RB; r++) {
+        if (!(R.held >> r & 1u)) continue;
+        float x[8];
+        q8_decode8(w[r], __uint_as_float(b[r] << 23), x);
+        q8_put8<DT>(is_v ? a.v_dst : a.k_dst,
+                    (static_cast<uint64_t>(R.row0 + r) * g.kv_heads + R.h) * g.head_dim + 8u * u, x);
+    }
 }
 
 uint32_t q8_seg_shift(uint32_t head_dim) {
@@ -175,12 +294,38 @@ Q8Geom q8_geom(const thb_pool* p, uint32_t layer, const thb_rows* rows, uint32_t
     return g;
 }
 
-// Workgroups of one operand (K or V) of m rows.
-uint32_t q8_wgs(const Q8Geom& g) {
-    const uint64_t vecs = static_cast<uint64_t>(g.m) * g.kv_heads, per = 4ull * (64u >> g.seg_shift);
+// Rows a lane handles: 4 where the call still has two waves per SIMD, which
+// fetch 4 rows each before they store the first.
+uint32_t q8_rows_per_lane(const Q8Geom& g, uint32_t cus) {
+    return (2ull * g.m * g.kv_heads << g.seg_shift) >= 64ull * 4 * 8 * cus ? 4u : 1u;
+}
+
+// Workgroups of one operand (K or V) of m rows, rb a lane.
+uint32_t q8_wgs(const Q8Geom& g, uint32_t rb) {
+    const uint64_t rows = rb > 1 ? static_cast<uint64_t>(g.m) + 2 * (rb - 1) : g.m;  // (groups are shifted by up to rb - 1)
+    const uint64_t vecs = rows / rb * g.kv_heads, per = 4ull * (64u >> g.seg_shift);
     const uint64_t n = (vecs + per - 1) / per;
-    if (vecs > 0x7FFFFFFFull || n > 0x3FFFFFFFull) throw HipError{hipErrorInvalidConfiguration, "append grid too large"};
+    if (static_cast<uint64_t>(g.m) * g.kv_heads > 0x7FFFFFFFull || n > 0x3FFFFFFFull)
+        throw HipError{hipErrorInvalidConfiguration, "append grid too large"};
     return static_cast<uint32_t>(n);
+}
+
+template <uint32_t DT>
+void store_rows(uint32_t rb, const Q8StoreArgs& a, hipStream_t s) {
+    const dim3 grid(2 * a.k_wgs);
+    if (rb == 4)
+        hipLaunchKernelGGL((q8_store_kernel<DT, 4>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((q8_store_kernel<DT, 1>), grid, dim3(256), 0, s, a);
+}
+
+template <uint32_t DT>
+void load_rows(uint32_t rb, const Q8LoadArgs& a, hipStream_t s) {
+    const dim3 grid(2 * a.k_wgs);
+    if (rb == 4)
+        hipLaunchKernelGGL((q8_load_kernel<DT, 4>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((q8_load_kernel<DT, 1>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -189,16 +334,16 @@ void launch_q8_store(thb_pool* p, uint32_t layer, const void* k_src, const void*
                      const thb_rope* rope, const thb_rows* rows, uint32_t row_off, uint32_t m, hipStream_t s) {
     Q8StoreArgs a;
     a.g = q8_geom(p, layer, rows, row_off, m);
+    const uint32_t rb = q8_rows_per_lane(a.g, p->cus);
     a.k_src = k_src;
     a.v_src = v_src;
-    a.k_wgs = q8_wgs(a.g);
+    a.k_wgs = q8_wgs(a.g, rb);
     a.rope_on = rope != nullptr;
     a.rope = rope ? rope_dev(*rope, false) : RopeDev{};
-    const dim3 grid(2 * a.k_wgs);
     switch (src_dtype) {
-        case THB_DT_F32: hipLaunchKernelGGL(q8_store_kernel<THB_DT_F32>, grid, dim3(256), 0, s, a); break;
-        case THB_DT_F16: hipLaunchKernelGGL(q8_store_kernel<THB_DT_F16>, grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL(q8_store_kernel<THB_DT_BF16>, grid, dim3(256), 0, s, a); break;
+        case THB_DT_F32: store_rows<THB_DT_F32>(rb, a, s); break;
+        case THB_DT_F16: store_rows<THB_DT_F16>(rb, a, s); break;
+        default: store_rows<THB_DT_BF16>(rb, a, s); break;
     }
     THB_HIP(hipGetLastError());
 }
@@ -207,14 +352,14 @@ void launch_q8_load(thb_pool* p, uint32_t layer, void* k_dst, void* v_dst, uint3
                     uint32_t row_off, uint32_t m, hipStream_t s) {
     Q8LoadArgs a;
     a.g = q8_geom(p, layer, rows, row_off, m);
+    const uint32_t rb = q8_rows_per_lane(a.g, p->cus);
     a.k_dst = k_dst;
     a.v_dst = v_dst;
-    a.k_wgs = q8_wgs(a.g);
-    const dim3 grid(2 * a.k_wgs);
+    a.k_wgs = q8_wgs(a.g, rb);
     switch (dst_dtype) {
-        case THB_DT_F32: hipLaunchKernelGGL(q8_load_kernel<THB_DT_F32>, grid, dim3(256), 0, s, a); break;
-        case THB_DT_F16: hipLaunchKernelGGL(q8_load_kernel<THB_DT_F16>, grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL(q8_load_kernel<THB_DT_BF16>, grid, dim3(256), 0, s, a); break;
+        case THB_DT_F32: load_rows<THB_DT_F32>(rb, a, s); break;
+        case THB_DT_F16: load_rows<THB_DT_F16>(rb, a, s); break;
+        default: load_rows<THB_DT_BF16>(rb, a, s); break;
     }
     THB_HIP(hipGetLastError());
 }
