@@ -12,8 +12,11 @@
 //    bf16 query is one exact f16 operand and an f32 or rotated one is split into
 //    a high and a low half (22 bits).
 //  * PV in bf16, whose exponents hold p_j 2^ev_j for any scale; the product is
-//    split into a high and a low half (16 bits, 2^-17 of each term).  The sum of
-//    the probabilities is kept in f32 from the unrounded ones.
+//    split into a high and a low part (16 bits, 2^-17 of each term) for a 16-bit
+//    output and a third (24 bits) for f32 (two leave 2e-6 to 3.4e-6 of an output's
+//    size, three under 1e-6; 1000 rows after 3000 keys at head_dim 256 159 / 170
+//    us, decode unchanged).  The sum of the probabilities is kept
+//    in f32 from the unrounded ones.
 #include <type_traits>
 
 #include "attn_decode.hpp"
@@ -47,18 +50,19 @@ __device__ __forceinline__ float q8_scale(uint32_t w, int e) {
     const uint32_t b = e == 0 ? w << 23 : e == 1 ? w << 15 : e == 2 ? w << 7 : w >> 1;
     return __uint_as_float(b & 0x7f800000u);
 }
-// High and low bf16 parts of 8 values.
-__device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8& h, bf16x8& l) {
+// N bf16 parts of 8 values, the highest first.
+template <int N>
+__device__ __forceinline__ void split_bf16(float (&x)[8], bf16x8 (&part)[N]) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-        const bf16x2 hh = __builtin_convertvector((f32x2{x[e], x[e + 1]}), bf16x2);
-        const bf16x2 ll = __builtin_convertvector(
-            (f32x2{x[e] - static_cast<float>(hh[0]), x[e + 1] - static_cast<float>(hh[1])}), bf16x2);
-        h[e] = hh[0];
-        h[e + 1] = hh[1];
-        l[e] = ll[0];
-        l[e + 1] = ll[1];
-    }
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const bf16x2 hh = __builtin_convertvector((f32x2{x[e], x[e + 1]}), bf16x2);
+            part[n][e] = hh[0];
+            part[n][e + 1] = hh[1];
+            x[e] -= static_cast<float>(hh[0]);
+            x[e + 1] -= static_cast<float>(hh[1]);
+        }
 }
 
 // The query operand of a lane (load_q_f32's elements) in f16, scaled by a power
@@ -105,7 +109,8 @@ struct Q8Lds {
 
 // One (group, partition, KV head) per workgroup of W waves, which split the
 // partition's keys into W runs of 32-key steps and keep NB steps in flight each.
-template <int HD, int W, int NB, bool QLO, bool FULL>
+// PP: bf16 parts of the probabilities.
+template <int HD, int W, int NB, bool QLO, int PP, bool FULL>
 __global__ __launch_bounds__(64 * W) void attn_q8(AttnArgs a) {
     constexpr int KS = HD / 32;  // QK k-steps of 32 dimensions
     constexpr int KB = HD / 64;  // 1 KiB blocks of a 16-key tile
@@ -242,15 +247,16 @@ __global__ __launch_bounds__(64 * W) void attn_q8(AttnArgs a) {
             // (A masked slot's scale may be anything.)
             p[e] = in[e] ? pe * q8_scale(x.s[e >> 2][1], e & 3) : 0.0f;
         }
-        bf16x8 ph, pl;
-        split_bf16(p, ph, pl);
+        bf16x8 part[PP];
+        split_bf16<PP>(p, part);
 #pragma unroll
         for (int j = 0; j < KB; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const bf16x8 vc = q8_bf16(x.v[0][j][i], x.v[1][j][i]);
-                o[4 * j + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, ph, o[4 * j + i], 0, 0, 0);
-                o[4 * j + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, pl, o[4 * j + i], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < PP; n++)
+                    o[4 * j + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, part[n], o[4 * j + i], 0, 0, 0);
             }
     };
 
@@ -809,18 +815,22 @@ __global__ __launch_bounds__(64 * kQ8PrefillWaves, NCG == 2 ? 2 : HD <= 64 ? 4 :
 
 bool args_query_lo(const AttnArgs& a) { return q8_query_lo(a.q_dt, a.rope_on); }
 
+template <int HD, bool QLO, int PP>
+void launch_q8_parts(dim3 grid, const AttnArgs& a, hipStream_t s) {
+    constexpr int W = q8_waves(HD), NB = q8_ring(HD);
+    if (a.full)
+        hipLaunchKernelGGL((attn_q8<HD, W, NB, QLO, PP, true>), grid, dim3(64 * W), 0, s, a);
+    else
+        hipLaunchKernelGGL((attn_q8<HD, W, NB, QLO, PP, false>), grid, dim3(64 * W), 0, s, a);
+}
+
 template <int HD>
 void launch_q8_hd(dim3 grid, const AttnArgs& a, hipStream_t s) {
-    constexpr int W = q8_waves(HD), NB = q8_ring(HD);
-    const bool lo = args_query_lo(a);
-    if (a.full && lo)
-        hipLaunchKernelGGL((attn_q8<HD, W, NB, true, true>), grid, dim3(64 * W), 0, s, a);
-    else if (a.full)
-        hipLaunchKernelGGL((attn_q8<HD, W, NB, false, true>), grid, dim3(64 * W), 0, s, a);
-    else if (lo)
-        hipLaunchKernelGGL((attn_q8<HD, W, NB, true, false>), grid, dim3(64 * W), 0, s, a);
+    const bool lo = args_query_lo(a), f32 = a.y_dt == THB_DT_F32;
+    if (lo)
+        f32 ? launch_q8_parts<HD, true, 3>(grid, a, s) : launch_q8_parts<HD, true, 2>(grid, a, s);
     else
-        hipLaunchKernelGGL((attn_q8<HD, W, NB, false, false>), grid, dim3(64 * W), 0, s, a);
+        f32 ? launch_q8_parts<HD, false, 3>(grid, a, s) : launch_q8_parts<HD, false, 2>(grid, a, s);
 }
 
 template <int HD, int NCG, bool QLO, bool PLO>
