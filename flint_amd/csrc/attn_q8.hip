@@ -65,6 +65,34 @@ __device__ __forceinline__ void split_bf16(float (&x)[8], bf16x8 (&part)[N]) {
         }
 }
 
+// Soft-capped scores, cap2 * tanh(y).  They are mostly small beside the cap, where
+// 1 - 2 / (exp(2y) + 1) would leave 2^-23 of the whole cap: below 1/4 the odd
+// Taylor polynomial (the next term is 2^-26 of y), and (1 - t) / (1 + t) of t =
+// exp(-2|y|) where some score of the wave is above.
+__device__ __forceinline__ void soft_cap(float (&y)[8], float cap2) {
+    float r[8];
+    bool big = false;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float y2 = y[e] * y[e];
+        float t = __builtin_fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f);
+        t = __builtin_fmaf(t, y2, 2.0f / 15.0f);
+        t = __builtin_fmaf(t, y2, -1.0f / 3.0f);
+        r[e] = __builtin_fmaf(t * y2, y[e], y[e]);
+        big = big || !(y2 < 0.0625f);
+    }
+    if (__builtin_amdgcn_ballot_w64(big) != 0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float t = fast_exp2(__builtin_fabsf(y[e]) * -2.8853900817779268f);  // -2 log2(e)
+            const float z = __builtin_copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), y[e]);
+            r[e] = y[e] * y[e] < 0.0625f ? r[e] : z;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = cap2 * r[e];
+}
+
 // The query operand of a lane (load_q_f32's elements) in f16, scaled by a power
 // of two and by pre (1 or -1); returns the factor that undoes the power of two.
 // Every lane must call it.
@@ -218,15 +246,15 @@ __global__ __launch_bounds__(64 * W) void attn_q8(AttnArgs a) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float y = s[u][e] * (q8_scale(x.s[u][0], e) * qf);
-                if (FULL && cap2 != 0.0f) y = cap2 * tanh_approx(y);
-                const uint32_t t = t0 + 16u * u + 4u * a4 + e;
-                in[4 * u + e] = t - clo < cspan;
-                y = in[4 * u + e] ? y : -INFINITY;
-                sv[4 * u + e] = y;
-                mx = fmaxf(mx, y);
-            }
+            for (int e = 0; e < 4; e++) sv[4 * u + e] = s[u][e] * (q8_scale(x.s[u][0], e) * qf);
+        if (FULL && cap2 != 0.0f) soft_cap(sv, cap2);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t t = t0 + 16u * (e >> 2) + 4u * a4 + (e & 3);
+            in[e] = t - clo < cspan;
+            sv[e] = in[e] ? sv[e] : -INFINITY;
+            mx = fmaxf(mx, sv[e]);
+        }
         // Lazy rescale: the running max moves only when a score beats it by
         // more than kTau.
         if (__builtin_amdgcn_ballot_w64(mx > m + kTau) != 0) {
@@ -639,8 +667,12 @@ __global__ __launch_bounds__(64 * kQ8PrefillWaves, NCG == 2 ? 2 : HD <= 64 ? 4 :
         for (int g = 0; g < NCG; g++) {
             kf[g] = fmaxf(qf[g] * kscale, 1.17549435e-38f);
             if constexpr (CAP) {
+                float y[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) sc[g][e >> 2][e & 3] = cap2 * tanh_approx(sc[g][e >> 2][e & 3] * kf[g]);
+                for (int e = 0; e < 8; e++) y[e] = sc[g][e >> 2][e & 3] * kf[g];
+                soft_cap(y, cap2);
+#pragma unroll
+                for (int e = 0; e < 8; e++) sc[g][e >> 2][e & 3] = y[e];
             }
             if constexpr (decltype(masked_t)::value) {
                 uint32_t t = ts + 4u * a4 - clo[g];
