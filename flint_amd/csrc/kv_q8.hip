@@ -72,8 +72,10 @@ __device__ inline uint32_t q8_seg_max(uint32_t m, uint32_t seg_shift) {
 }
 
 // Rows of a segment: RB consecutive ones of one head.  Groups of RB rows start
-// where the first row's slot would be a multiple of RB, so that those of a chunk
-// of consecutive tokens cover whole groups of RB slots.
+// where slots do that are a multiple of RB, in the chunk that the call begins with
+// or, if its first two rows are no chunk, ends with (64 decode rows and 8 chunks of
+// 512: 10 us to append, 15 to read back, 20 with groups that start inside the
+// chunks' groups of slots, as those of chunks elsewhere in a call may).
 template <uint32_t RB>
 struct Q8Rows {
     uint32_t u, h, row0;          // the lane's unit of 8 dims, head, first row (may be "negative")
@@ -87,7 +89,12 @@ struct Q8Rows {
         const uint32_t i = (bid * 4 + (threadIdx.x >> 6)) * (64u >> g.seg_shift) + (lane >> g.seg_shift);
         const uint32_t gr = i / g.kv_heads;
         h = i - gr * g.kv_heads;
-        row0 = gr * RB - (RB > 1 ? g.meta[0] & (RB - 1u) : 0u);
+        row0 = gr * RB;
+        if (RB > 1 && g.m > 1) {
+            const bool first = g.meta[8] == g.meta[0] + 1u;
+            const uint32_t r = first ? 0u : g.m - 1u;
+            row0 -= (g.meta[8 * r] - r) & (RB - 1u);
+        }
         on = held = 0;
         run = RB > 1;
 #pragma unroll
