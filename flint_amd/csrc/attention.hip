@@ -1875,7 +1875,8 @@ void launch_merge(uint32_t hd_t, dim3 grid, const AttnArgs& a, hipStream_t s) {
     }
 }
 
-int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, bool blocks_ok, bool q_lo, AttnPlan& plan) {
+int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, uint32_t hd, bool blocks_ok, bool q_lo,
+               AttnPlan& plan) {
     const Arena& arena = pool->arena.a;
     const uint32_t m = sp.m;
     const uint32_t* args = rows->host.data() + 8 * static_cast<size_t>(sp.row_off);
@@ -1900,28 +1901,45 @@ int build_plan(thb_pool* pool, const thb_rows* rows, const thb_attn_spec& sp, ui
     const uint32_t PL = pool->part_len;
     const uint32_t hd_t = template_hd(hd);
     const bool q8 = is_q8(pool), wide = !q8 && prefill_wide(hd_t);
-    const uint32_t WB = q8 ? (blocks_ok && hd_t <= kQ8PrefillHd ? kQ8PrefillWaves : 0u) : block_groups(wide, hd_t);  // query groups per prefill block
+    // query groups per prefill block
+    const uint32_t WB = q8 ? (blocks_ok && hd_t <= kQ8PrefillHd ? kQ8PrefillWaves : 0u) : block_groups(wide, hd_t);
     const uint32_t align = std::max<uint32_t>(pool->page_len, 16);
-    QueryPlan qp = plan_groups(rp, G, PL, align, WB);
-    if (q8 && WB) {
-        // Over an 8-bit pool blocks pay from one workgroup per CU on; with fewer their
-        // groups run on the decode kernel, which converts the codes itself but puts each
-        // group on a workgroup of 8 waves (8 KV heads of 128 x 4, us as decode items /
-        // blocks: 512 fresh rows 24.9 / 23.8, 768 39.8 / 31.2, 1024 58.7 / 39.0, 256
-        // after 16000 keys 240 / 165; 32 after 8000 keys 40 / 95).  head_dim 256 stays
-        // there (8 x 2 x 256, 1000 rows after 3000 keys 154 / 210).  From two rounds of
-        // workgroups on, two groups a wave (4096 rows 210 -> 191, 8192 854 -> 779, but
+    QueryPlan qp;
+    if (!q8 || !WB) {
+        qp = plan_groups(rp, G, PL, align, WB);
+    } else {
+        // Over an 8-bit pool blocks pay where a chunk's groups share the cost of the
+        // expanded keys, and from one workgroup per CU on; other groups run on the decode
+        // kernel, which converts the codes itself but puts each group on a workgroup of 8
+        // waves.  8 KV heads of 128 x 4, us as decode items / blocks: 32 sequences of 1000
+        // keys, 4 groups each, 54 / 70, 8 groups 110 / 76; of 8192 keys, whose expansion
+        // does not fit the 256 MiB behind L2, 4 groups 267 / 532, 8 502 / 690, 16 1003 /
+        // 1080; 16 of 4000 keys, 32 groups, 597 / 370.  512 fresh rows 24.9 / 23.8, 768
+        // 39.8 / 31.2, 1024 58.7 / 39.0, 256 after 16000 keys 240 / 165.  head_dim 256
+        // stays there (8 x 2 x 256, 1000 rows after 3000 keys 154 / 210).  From four rounds
+        // of workgroups on, two groups a wave (4096 rows 210 -> 191, 8192 854 -> 779, but
         // 2048 73 -> 86): not beside a query's low halves, whose registers they would take.
-        auto wgs = [&](const QueryPlan& q) {
+        auto wgs = [&] {
             uint64_t n = 0;
-            for (size_t b = 0; b < q.blocks.size(); b += kBlockWords) n += q.blocks[b + 5];
+            for (size_t b = 0; b < qp.blocks.size(); b += kBlockWords) n += qp.blocks[b + 5];
             return n * pool->kv_heads;
         };
-        const uint64_t n = wgs(qp);
-        if (n < pool->cus)
+        auto scratch = [&] {  // at most: a sequence's last key among its blocks
+            std::map<uint32_t, uint32_t> end;
+            for (size_t b = 0; b < qp.blocks.size(); b += kBlockWords)
+                end[qp.blocks[b + 2]] = std::max(end[qp.blocks[b + 2]], qp.blocks[b + 4]);
+            uint64_t steps = 0;
+            for (auto& e : end) steps += (uint64_t(e.second) + 31) / 32;
+            return steps * q8_step_bytes(hd_t) * pool->kv_heads;
+        };
+        uint32_t min_groups = 8;
+        qp = plan_groups(rp, G, PL, align, WB, min_groups);
+        if (scratch() > kQ8CachedScratch) qp = plan_groups(rp, G, PL, align, WB, min_groups = 16);
+        const uint64_t n = wgs();
+        if (n < pool->cus || scratch() > kQ8MaxScratch)
             qp = plan_groups(rp, G, PL, align, 0);
         else if (n >= 8ull * pool->cus && hd_t == 128 && !q_lo)
-            qp = plan_groups(rp, G, PL, align, 2 * WB);
+            qp = plan_groups(rp, G, PL, align, 2 * WB, min_groups);
     }
     auto& groups = qp.groups;
     auto& blocks = qp.blocks;

@@ -75,7 +75,8 @@ struct QueryPlan {
 // parts empty): a function of its own key range only.  G: query heads per KV
 // head; PL: part_len; align: a part's length is a multiple of it; WB: query
 // groups per block (0: no blocks).
-inline QueryPlan plan_groups(const RowPlan& rp, uint32_t G, uint32_t PL, uint32_t align, uint32_t WB) {
+inline QueryPlan plan_groups(const RowPlan& rp, uint32_t G, uint32_t PL, uint32_t align, uint32_t WB,
+                             uint32_t min_groups = 4) {
     QueryPlan qp;
     auto& groups = qp.groups;
     auto& blocks = qp.blocks;
@@ -106,7 +107,7 @@ inline QueryPlan plan_groups(const RowPlan& rp, uint32_t G, uint32_t PL, uint32_
         partition(lo, hi, base, n_parts, plen);
         groups.insert(groups.end(), {r0, R, h0, H, seq, lo, hi, n_parts, base, plen, 0u});
     };
-    // A chunk that needs at least 4 groups (a prefill chunk) is cut into
+    // A chunk that needs at least min_groups groups (a prefill chunk) is cut into
     // blocks of WB consecutive groups for attn_prefill; the others go to the
     // decode kernel.
     for (auto& c : rp.chunks) {
@@ -121,7 +122,7 @@ inline QueryPlan plan_groups(const RowPlan& rp, uint32_t G, uint32_t PL, uint32_
         }
         const uint32_t ncg = static_cast<uint32_t>(groups.size() / kGroupWords) - first;
         in_block.resize(first + ncg, 0);
-        if (G > kCols || ncg < 4 || WB == 0) continue;
+        if (G > kCols || ncg < min_groups || WB == 0) continue;
         for (uint32_t b = 0; b < ncg; b += WB) {
             const uint32_t g0 = first + b, ng = std::min(WB, ncg - b);
             uint32_t lo = 0xFFFFFFFFu, hi = 0;

@@ -1,5 +1,5 @@
-"""Chunks over 8-bit pages large enough for prefill blocks (one workgroup per
-CU: many KV heads and short partitions here), and appends large enough for four
+"""Chunks over 8-bit pages large enough for prefill blocks (8 query groups, one
+workgroup per CU: many KV heads and short partitions here), and appends large enough for four
 rows a lane, against 64 bits."""
 
 import ctypes
@@ -41,6 +41,9 @@ BLOCKS = [
     (32, 16, 128, 16, [(400, 150)], "f32", "f32", 0, 30.0, 64),
     (32, 16, 80, 64, [(401, 150)], "f16", "f16", 37, 30.0, 64),
     (48, 16, 64, 16, [(350, 33)] * 6, "f16", "f32", 0, 20.0, 128),
+    (32, 32, 64, 16, [(300, 140)], "f32", "f32", 0, 0.0, 64),
+    (32, 32, 96, 16, [(300, 140)], "f32", "f16", 0, 0.0, 64),
+    (48, 16, 64, 16, [(350, 60), (40, 5), (90, 90), (200, 50), (90, 60), (333, 60)], "f16", "f32", 0, 20.0, 128),
     # two query groups a wave: eight times the workgroups
     (256, 64, 128, 16, [(260, 64)], "f16", "f16", 0, 0.0, 32),
     (256, 64, 128, 16, [(260, 64)], "bf16", "f32", 0, 25.0, 32),
@@ -80,7 +83,7 @@ def test_scales_from_step_to_step(torch_cuda, hd, qd, yd):
     """Scales of V that rise and fall by 2^60 from one run of 32 keys to the next,
     zero keys and values among them."""
     torch = torch_cuda
-    n, new, nkv, nq = 384, 100, 32, 32
+    n, new, nkv, nq = 384, 150, 32, 32
     f = Filled(torch, [n], nkv, hd, part_len=128)
     g = f.g
     k, v = _kv(torch, g, n, nkv, hd, torch.float32)
@@ -107,7 +110,7 @@ def test_scales_from_step_to_step(torch_cuda, hd, qd, yd):
 def test_nan_in_blocks(torch_cuda, hd, new):
     """A NaN token reaches the rows of its chunk that read it and no other."""
     torch = torch_cuda
-    n, nkv, nq = 200, 64, 64
+    n, nkv, nq = 200, 64, 128
     f = Filled(torch, [n], nkv, hd, part_len=64, budget=[n + 64])
     pos = list(range(n - new, n))
     bad = n - new + new // 2
@@ -132,7 +135,7 @@ def test_slots_behind_the_chunk(torch_cuda):
     """What the slots behind the last key hold (a longer sequence's huge and NaN
     vectors, on pages since reused) does not touch a chunk's precision."""
     torch = torch_cuda
-    n, new, nkv, hd = 203, 100, 32, 128
+    n, new, nkv, hd = 203, 150, 32, 128
     pool = make_pool([n + 53], nkv, hd, page_len=16, kv_dtype="e4m3", part_len=64)
     pool.alloc(0, 0, n + 53)
     g = torch.Generator(device="cuda").manual_seed(1)
