@@ -156,9 +156,9 @@ constexpr uint32_t kQ8PrefillHd = 128;  // the largest head_dim that has prefill
 // Scratch of a call's prefill blocks: per KV head and step of 32 keys the expanded
 // codes and a Q8Ref (attn_q8.hip).
 constexpr uint32_t kQ8RefBytes = 32, kQ8RegionWords = 4;
-// What of it stays close to the CUs, and what a call takes at most.
-constexpr uint64_t kQ8CachedScratch = 256ull << 20, kQ8MaxScratch = 2ull << 30;
 constexpr uint64_t q8_step_bytes(uint32_t hd_t) { return 128ull * hd_t + kQ8RefBytes; }
+// Scratch that stays in the cache behind L2, and what a call takes at most.
+constexpr uint64_t kQ8CachedScratch = 256ull << 20, kQ8MaxScratch = 2ull << 30;
 
 namespace {
 

@@ -83,6 +83,10 @@ extern "C" {
  *  - thb_kv_load reads values back; thb_kv_gather, thb_kv_scatter and their
  *    batched forms, which move 16-bit words, are refused (THB_ERR_CONFIG);
  *  - attention, the page API, forks and block copies work as on any pool;
+ *    chunks of many rows first expand their keys into scratch memory of the pool
+ *    (4 bytes per key, KV head and dim, at most 2 GiB a call), and which of two
+ *    kernels runs a chunk depends on the whole call, so that its last bits may
+ *    differ from those of the chunk alone (decode rows' do not);
  *  - device plans are fixed-grid ones without an append (flags 0). */
 #define THB_KV_E4M3 2u
 
