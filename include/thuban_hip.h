@@ -86,7 +86,9 @@ extern "C" {
  *    chunks of many rows first expand their keys into scratch memory of the pool
  *    (4 bytes per key, KV head and dim, at most 2 GiB a call), and which of two
  *    kernels runs a chunk depends on the whole call, so that its last bits may
- *    differ from those of the chunk alone (decode rows' do not);
+ *    differ from those of the chunk alone (decode rows' do not).  Expanded
+ *    codes are exact down to 2^-22 of the largest scale among 32 consecutive
+ *    keys, and off by at most 2^-40 of that key's largest value below it;
  *  - device plans are fixed-grid ones without an append (flags 0). */
 #define THB_KV_E4M3 2u
 
